@@ -104,11 +104,19 @@ SIGNATURES: dict[str, list] = {
     "halo_b200_axpy_slot": [_p, _p, _p, _u32, _u32],
     "halo_b200_moe_combine_ex": [_p, _i, _p, _p, _p, _i, _p, _p, _i, _u32, _u32, _u32],
     "halo_b200_embed_q8_0_ex": [_p, _u64, _u32, _p, _u32, _u32, _u32, _p, _i, _u32],
+    "halo_b200_paged_plan": [_p, _u64, _u32, _p, _p, _p, _u32, _u32, _p, _p, _p, _p, _p, _u32, _u32],
+    "halo_b200_paged_store": [_p, _u64, _u64, _p, _u64, _u64, _i, _p, _p, _i, _u64, _u64, _u64, _u32, _u32, _p, _u32, _u32,
+                              _u32],
+    "halo_b200_attention_packed": [_p, _u64, _u64, _p, _u64, _u64, _p, _u64, _u64, _p, _u64, _u64, _i, _p, _u32, _u32, _u32,
+                                   _u32, _u32, _f, _i, _p, _p, _u64],
+    "halo_b200_attention_paged": [_p, _u64, _u64, _p, _p, _u64, _u64, _u64, _u32, _u32, _p, _u64, _u32, _p, _p, _u64, _u64,
+                                  _i, _p, _u32, _u32, _u32, _u32, _u32, _f, _i, _p, _p, _u64],
 }
 
 # Entry points with other calling shapes.
 OTHER_EXPORTS = ["halo_b200_version", "halo_b200_launch", "halo_b200_kernel_count", "halo_b200_kernel_name",
-                 "halo_b200_tune", "halo_b200_conv_stage_timeouts", "halo_b200_stage_timeouts"]
+                 "halo_b200_tune", "halo_b200_conv_stage_timeouts", "halo_b200_stage_timeouts",
+                 "halo_b200_attention_workspace"]
 
 
 class HaloArgValue(C.Union):
@@ -144,6 +152,8 @@ class Library:
         self.cdll.halo_b200_kernel_count.argtypes = []
         self.cdll.halo_b200_kernel_name.restype = C.c_char_p
         self.cdll.halo_b200_kernel_name.argtypes = [_sz]
+        self.cdll.halo_b200_attention_workspace.restype = _u64
+        self.cdll.halo_b200_attention_workspace.argtypes = [_u32]
         self.cdll.halo_b200_tune.restype = C.c_int
         self.cdll.halo_b200_tune.argtypes = [C.c_char_p, C.c_int]
         self.cdll.halo_b200_launch.restype = C.c_int

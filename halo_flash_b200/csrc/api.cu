@@ -190,6 +190,35 @@ int RunQuant(QuantArgs a, const char* what, halo_b200_stream stream, char* err, 
   return Done(LaunchQuantize(a, S(stream)), what, err, errlen);
 }
 
+bool ValidPage(uint32_t page_size) { return page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
+uint32_t Log2(uint32_t v) {
+  uint32_t s = 0;
+  while (v >>= 1) ++s;
+  return s;
+}
+
+int RunAttention(AttnArgs a, uint64_t workspace_bytes, const char* what, halo_b200_stream stream, char* err, size_t errlen) {
+  if (a.tokens == 0 || a.batch == 0) return Done(cudaSuccess, what, err, errlen);  // an empty step is a no-op
+  REQUIRE(a.q && a.k && a.v && a.out && a.cu, "%s: null pointer", what);
+  REQUIRE(a.dtype == kF16 || a.dtype == kBF16, "%s: dtype must be fp16 or bf16", what);
+  REQUIRE(a.dim > 0 && a.dim <= 256 && a.dim % 8 == 0, "%s: dim %u must be a multiple of 8 up to 256", what, a.dim);
+  REQUIRE(a.kv_heads > 0 && a.q_heads > 0 && a.q_heads % a.kv_heads == 0, "%s: q_heads %u is no multiple of kv_heads %u", what,
+          a.q_heads, a.kv_heads);
+  REQUIRE(a.q_heads / a.kv_heads <= 128, "%s: more than 128 query heads for each K/V head", what);
+  REQUIRE(std::isfinite(a.scale) && a.scale > 0.0f, "%s: scale must be positive and finite", what);
+  REQUIRE(a.causal == 0 || a.causal == 1, "%s: causal must be 0 or 1", what);
+  REQUIRE(a.tokens < (1u << 31) && a.batch < (1u << 31), "%s: more than 2^31 tokens or sequences", what);
+  REQUIRE(Aligned(a.q, 16) && Aligned(a.k, 16) && Aligned(a.v, 16) && Aligned(a.out, 16), "%s: pointer not 16-byte aligned", what);
+  REQUIRE(Aligned(a.cu, 4) && Aligned(a.kv_len, 4) && Aligned(a.table, 4) && Aligned(a.lse, 4),
+          "%s: pointer not aligned to its element type", what);
+  const uint64_t strides[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.k_page, a.v_row, a.v_head, a.v_page, a.out_row, a.out_head};
+  for (const uint64_t v : strides) REQUIRE(v % 8 == 0 && v < (uint64_t{1} << 38), "%s: strides must be multiples of 8", what);
+  REQUIRE(a.workspace && Aligned(a.workspace, 16), "%s: the workspace is null or not 16-byte aligned", what);
+  REQUIRE(workspace_bytes >= AttentionWorkspaceBytes(a.dim), "%s: the workspace has %llu bytes, %llu are needed", what,
+          static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(AttentionWorkspaceBytes(a.dim)));
+  return Done(LaunchAttention(a, S(stream)), what, err, errlen);
+}
+
 // check_only: validate and return 0 when the vector kernels (and with them the rotation-table form) can run these
 // arguments, 1 when only the unfused fallback can, -1 with a message when the call is invalid; nothing is launched.
 int RunNormRope(NormRopeArgs a, float theta, const char* what, halo_b200_stream stream, char* err, size_t errlen,
@@ -1480,10 +1509,11 @@ int halo_b200_scale_silu(halo_b200_stream stream, const float* x, void* y, int y
 
 int halo_b200_stage_timeouts(unsigned int* count, char* err, size_t errlen) {
   REQUIRE(count != nullptr, "halo_b200_stage_timeouts: count is null");
-  unsigned int conv = 0, rope = 0;
+  unsigned int conv = 0, rope = 0, attn = 0;
   cudaError_t e = ReadConvStageTimeouts(&conv);
   if (e == cudaSuccess) e = ReadRopeStageTimeouts(&rope);
-  *count = conv + rope;
+  if (e == cudaSuccess) e = ReadAttentionTimeouts(&attn);
+  *count = conv + rope + attn;
   return Done(e, "halo_b200_stage_timeouts", err, errlen);
 }
 
@@ -1547,5 +1577,164 @@ int halo_b200_axpy_slot(halo_b200_stream stream, float* y, const float* x, const
   return RunMoeCombine(a, "halo_axpy_slot", stream, err, errlen);
 }
 
+
+// ---- paged K/V cache and attention -------------------------------------------------------------------
+int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table_stride, uint32_t table_cols,
+                         const uint32_t* past, const uint32_t* fresh, const int32_t* free_pages, uint32_t n_free,
+                         uint32_t page_size, int64_t* slot, uint32_t* pos, uint32_t* cu, uint32_t* kv_len,
+                         uint32_t* status, uint32_t batch, uint32_t tokens, char* err, size_t errlen) {
+  const char* what = "halo_paged_plan";
+  REQUIRE(ValidPage(page_size), "%s: page size %u must be a power of two in 8 .. 256", what, page_size);
+  REQUIRE(batch <= kMaxPlanBatch, "%s: more than %u requests", what, kMaxPlanBatch);
+  REQUIRE(batch == 0 || (past && fresh), "%s: null pointer", what);
+  REQUIRE(batch == 0 || table_cols == 0 || table, "%s: the table is null", what);
+  REQUIRE(tokens == 0 || slot, "%s: slot is null", what);
+  REQUIRE(n_free == 0 || free_pages, "%s: the free list is null", what);
+  REQUIRE(n_free < (1u << 31) && tokens < (1u << 31), "%s: more than 2^31 pages or tokens", what);
+  REQUIRE(table_stride >= table_cols || batch <= 1, "%s: table rows overlap", what);
+  REQUIRE(Aligned(table, 4) && Aligned(past, 4) && Aligned(fresh, 4) && Aligned(free_pages, 4) && Aligned(slot, 8) &&
+              Aligned(pos, 4) && Aligned(cu, 4) && Aligned(kv_len, 4) && Aligned(status, 4),
+          "%s: pointer not aligned to its element type", what);
+  if (batch == 0 && tokens == 0 && !cu && !status) return Done(cudaSuccess, what, err, errlen);
+  PlanArgs a{};
+  a.table = table;
+  a.table_stride = table_stride;
+  a.table_cols = table_cols;
+  a.past = past;
+  a.fresh = fresh;
+  a.free_pages = free_pages;
+  a.n_free = n_free;
+  a.page_shift = Log2(page_size);
+  a.batch = batch;
+  a.tokens = tokens;
+  a.slot = slot;
+  a.pos = pos;
+  a.cu = cu;
+  a.kv_len = kv_len;
+  a.status = status;
+  return Done(LaunchPagedPlan(a, S(stream)), what, err, errlen);
+}
+
+int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row_stride, uint64_t k_head_stride,
+                          const void* v, uint64_t v_row_stride, uint64_t v_head_stride, int dtype, void* k_cache,
+                          void* v_cache, int cache_dtype, uint64_t page_stride, uint64_t row_stride,
+                          uint64_t head_stride, uint32_t pages, uint32_t page_size, const int64_t* slot,
+                          uint32_t heads, uint32_t dim, uint32_t tokens, char* err, size_t errlen) {
+  const char* what = "halo_paged_store";
+  REQUIRE(ValidPage(page_size), "%s: page size %u must be a power of two in 8 .. 256", what, page_size);
+  REQUIRE(ValidDType(dtype) && ValidDType(cache_dtype), "%s: unknown dtype", what);
+  if (tokens == 0 || heads == 0 || dim == 0) return Done(cudaSuccess, what, err, errlen);
+  REQUIRE(k && v && k_cache && v_cache && slot, "%s: null pointer", what);
+  REQUIRE(static_cast<uint64_t>(heads) * dim < (1u << 31), "%s: rows of more than 2^31 values", what);
+  const size_t ss = DTypeSize(dtype), ds = DTypeSize(cache_dtype);
+  REQUIRE(Aligned(k, ss) && Aligned(v, ss) && Aligned(k_cache, ds) && Aligned(v_cache, ds) && Aligned(slot, 8),
+          "%s: pointer not aligned to its element type", what);
+  StoreArgs a{};
+  a.src[0] = k;
+  a.src[1] = v;
+  a.dst[0] = k_cache;
+  a.dst[1] = v_cache;
+  a.src_dtype = dtype;
+  a.dst_dtype = cache_dtype;
+  a.src_row[0] = k_row_stride;
+  a.src_row[1] = v_row_stride;
+  a.src_head[0] = k_head_stride;
+  a.src_head[1] = v_head_stride;
+  a.page_stride = page_stride;
+  a.row_stride = row_stride;
+  a.head_stride = head_stride;
+  a.slot = slot;
+  a.tokens = tokens;
+  a.heads = heads;
+  a.dim = dim;
+  a.page_shift = Log2(page_size);
+  a.pages = pages;
+  const uint64_t odd = k_row_stride | k_head_stride | v_row_stride | v_head_stride | page_stride | row_stride | head_stride | dim;
+  a.vec = odd % 8 == 0 && Aligned(k, 16) && Aligned(v, 16) && Aligned(k_cache, 16) && Aligned(v_cache, 16);
+  const cudaError_t e = LaunchPagedStore(a, S(stream));
+  if (e == cudaErrorInvalidValue) return Fail(err, errlen, "%s: unsupported (rows, cache) dtype combination", what);
+  return Done(e, what, err, errlen);
+}
+
+uint64_t halo_b200_attention_workspace(uint32_t dim) { return AttentionWorkspaceBytes(dim); }
+
+int halo_b200_attention_packed(halo_b200_stream stream, const void* q, uint64_t q_row_stride, uint64_t q_head_stride,
+                               const void* k, uint64_t k_row_stride, uint64_t k_head_stride, const void* v,
+                               uint64_t v_row_stride, uint64_t v_head_stride, void* out, uint64_t out_row_stride,
+                               uint64_t out_head_stride, int dtype, const uint32_t* cu, uint32_t batch,
+                               uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t dim, float scale,
+                               int causal, float* lse, void* workspace, uint64_t workspace_bytes, char* err,
+                               size_t errlen) {
+  AttnArgs a{};
+  a.q = q;
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.k = k;
+  a.k_row = k_row_stride;
+  a.k_head = k_head_stride;
+  a.v = v;
+  a.v_row = v_row_stride;
+  a.v_head = v_head_stride;
+  a.dtype = dtype;
+  a.cu = cu;
+  a.batch = batch;
+  a.tokens = tokens;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.scale = scale;
+  a.causal = causal;
+  a.out = out;
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.lse = lse;
+  a.workspace = workspace;
+  return RunAttention(a, workspace_bytes, "halo_attention_packed", stream, err, errlen);
+}
+
+int halo_b200_attention_paged(halo_b200_stream stream, const void* q, uint64_t q_row_stride, uint64_t q_head_stride,
+                              const void* k_cache, const void* v_cache, uint64_t page_stride, uint64_t row_stride,
+                              uint64_t head_stride, uint32_t pages, uint32_t page_size, const int32_t* table,
+                              uint64_t table_stride, uint32_t table_cols, const uint32_t* kv_len, void* out,
+                              uint64_t out_row_stride, uint64_t out_head_stride, int dtype, const uint32_t* cu,
+                              uint32_t batch, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t dim,
+                              float scale, int causal, float* lse, void* workspace, uint64_t workspace_bytes,
+                              char* err, size_t errlen) {
+  const char* what = "halo_attention_paged";
+  REQUIRE(ValidPage(page_size), "%s: page size %u must be a power of two in 8 .. 256", what, page_size);
+  REQUIRE(tokens == 0 || batch == 0 || (table && kv_len), "%s: null pointer", what);
+  REQUIRE(tokens == 0 || batch == 0 || pages > 0, "%s: the cache has no pages", what);
+  REQUIRE(pages < (1u << 31), "%s: more than 2^31 pages", what);
+  AttnArgs a{};
+  a.q = q;
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.k_row = a.v_row = row_stride;
+  a.k_head = a.v_head = head_stride;
+  a.k_page = a.v_page = page_stride;
+  a.pages = pages;
+  a.page_shift = Log2(page_size);
+  a.dtype = dtype;
+  a.table = table;
+  a.table_stride = table_stride;
+  a.table_cols = table_cols;
+  a.kv_len = kv_len;
+  a.cu = cu;
+  a.batch = batch;
+  a.tokens = tokens;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.scale = scale;
+  a.causal = causal;
+  a.out = out;
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.lse = lse;
+  a.workspace = workspace;
+  return RunAttention(a, workspace_bytes, what, stream, err, errlen);
+}
 
 }  // extern "C"

@@ -1,0 +1,952 @@
+// Attention over packed prompts and over a paged K/V cache, one kernel for both, for prompts, chunks and single
+// tokens: O = softmax(scale Q K^T + mask) V with grouped heads.
+//
+// Mathematics. A tile is 128 query rows against KT keys. S = Q K^T goes to TMEM in fp32; each row keeps a
+// reference r (near its running maximum) and l = sum of p, p = 2^(c s - c r), c = scale log2 e; O += P V stays in
+// TMEM in fp32, and at the end O / l is rounded once. Any reference gives the same result, so r follows the maximum
+// only when that has grown by more than 2^8: until then p stays below 2^8, which neither bf16 nor fp16 nor the fp32
+// sums mind, and O need not be rescaled. P is rounded to the inputs' 16-bit type for the tensor cores (as every
+// output is), l is summed from the unrounded p.
+//
+// Rows. The group of query heads that share a K/V head is folded into the rows: row r of a tile is token r / G, head
+// r % G, so one token of a group of eight already fills eight rows and K and V are read once for all heads.
+//
+// Work. A job is one (sequence, K/V head, row tile), costing its number of key tiles plus kJobCost. The jobs in their
+// order form one line of cost W, and every CTA takes an equal piece of that line: a job that a border cuts is
+// computed in pieces, whose unnormalized sums a second kernel joins. One rule thus balances a prompt's triangle,
+// ragged batches, and one long sequence that must be split over the whole GPU. No host knowledge of the lengths is
+// needed; every CTA finds its piece from cu / kv_len by itself.
+//
+// Roles in a CTA (384 threads): warp 8 copies Q, K and V by TMA into shared memory (K and V through a ring of
+// stages), warp 9 issues the tcgen05.mma, warps 0-3 and 4-7 are two softmax groups that take alternate key tiles
+// (thread = row), so that one group's exponentials run beside the other's TMEM traffic and the tensor cores.
+//
+// Waits are bounded as in stage.cuh: one that runs out sets a flag that makes the other waits return at once, the CTA
+// finishes its control flow without storing, and the count is reported by halo_b200_stage_timeouts.
+#include "attention.cuh"
+
+#include "common.cuh"
+#include "stage.cuh"
+
+namespace halo_b200 {
+
+namespace {
+
+__device__ unsigned int g_attn_timeouts = 0;
+
+constexpr uint32_t kRows = kAttnRows;
+constexpr uint32_t kThreads = 384;
+// Registers: three warpgroups of 168 at launch; the copying and multiplying one gives 80 a thread to the softmax
+// groups, which hold a whole row of S: 2 x 128 x 208 + 128 x 88 = 384 x 168.
+constexpr uint32_t kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "a share above the launch's total would wait for good");
+constexpr uint32_t kJobCost = 2;   // what a job costs beside its key tiles, in key tiles
+constexpr uint32_t kSnap = 1;      // a border within so many tiles of a job's end moves to that end
+constexpr uint32_t kMinShare = 3;  // least piece of work of a CTA
+constexpr uint32_t kMaxCtas = 148;
+constexpr float kLazy = 8.0f;      // log2 of the growth that a reference may lag behind
+constexpr uint32_t kTmemO = 256;   // TMEM columns: S0 0.., S1 128.., O 256..
+
+template <int D>
+struct Shape {
+  static constexpr uint32_t kKeys = D == 256 ? 64 : 128;        // keys of a tile
+  static constexpr uint32_t kStageBytes = kKeys * D * 2;        // 32, 32, 16 KB
+  static constexpr uint32_t kQBytes = kRows * D * 2;
+  static constexpr uint32_t kStages = D == 256 ? 5 : D == 128 ? 6 : 8;
+};
+
+struct alignas(16) Shared {
+  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_empty, m_full[2][4];
+  uint32_t tmem, abort;
+  uint32_t start[4], end[4];  // (sequence, K/V head, row tile, key tile) of the piece's borders
+  float m[2][kRows];
+  float l[2][kRows];
+};
+template <int D>
+constexpr uint32_t kSmemBytes = Shape<D>::kQBytes + Shape<D>::kStages * Shape<D>::kStageBytes + static_cast<uint32_t>(sizeof(Shared));
+static_assert(kSmemBytes<256> <= 232448 && kSmemBytes<128> <= 232448 && kSmemBytes<64> <= 232448, "shared memory of an SM");
+
+// ---- PTX ----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void bar_init(unsigned long long* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(unsigned long long* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(unsigned long long* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// 32 columns of this warp's 32 TMEM lanes. The results are only valid after tc_wait_ld().
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// The waits name the registers of the loads, so that no use of them can move ahead of the wait.
+#define HALO_R32(v)                                                                                                       \
+  "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),  \
+      "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), \
+      "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), \
+      "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+__device__ __forceinline__ void tc_wait_ld(float (&v)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : HALO_R32(v)::"memory"); }
+template <uint32_t N>
+__device__ __forceinline__ void tc_wait_ld(float (&v)[N][32]) {
+  tc_wait_ld(v[0]);
+#pragma unroll
+  for (uint32_t i = 1; i < N; ++i) asm volatile("" : HALO_R32(v[i])::"memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand with 128-byte swizzle (layout type 2, version 1): rows of 128 bytes in groups of eight, 1024
+// bytes apart; `lead` is the distance of the next 64 columns, which only an operand contiguous along its M / N axis uses.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) | (static_cast<uint64_t>(1024u >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulator, A and B both fp16 or both bf16; b_mn: B is contiguous along N.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instr_desc(uint32_t m, uint32_t n, bool b_mn) {
+  const uint32_t fmt = sizeof(T) == 2 && __is_same(T, bf16) ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// A bounded wait; a thread whose wait runs out tells the others.
+__device__ __forceinline__ void wait(Shared& sh, unsigned long long* b, uint32_t parity) {
+  const uint32_t bar = smem_addr(b);
+  uint32_t done = 0;
+  for (uint32_t spin = 0; spin < kStageSpinLimit && !done; ++spin) {
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (!done && spin >= 64) {
+      if (*reinterpret_cast<volatile uint32_t*>(&sh.abort)) return;
+      if (spin >= 4096) __nanosleep(256);
+    }
+  }
+  if (!done && atomicExch(&sh.abort, 1u) == 0) atomicAdd(&g_attn_timeouts, 1u);
+}
+__device__ __forceinline__ bool aborted(Shared& sh) { return *reinterpret_cast<volatile uint32_t*>(&sh.abort) != 0; }
+
+// ---- the line of work -----------------------------------------------------------------------------------------
+struct Seq {
+  uint32_t row0, rows;  // its query rows
+  uint32_t len;         // its keys
+  int off;              // row i sees keys [0, off + i + 1) when causal
+  uint32_t tiles;       // row tiles
+};
+__device__ __forceinline__ Seq load_seq(const AttnCall& c, uint32_t b, uint32_t tq) {
+  Seq s;
+  // lengths that do not fit the buffers are cut, so that no access leaves them
+  const uint32_t a0 = min(c.cu[b], c.tokens), a1 = min(c.cu[b + 1], c.tokens);
+  s.row0 = a0;
+  s.rows = a1 > a0 ? a1 - a0 : 0u;
+  s.len = s.rows;
+  if (c.kv_len) {
+    const unsigned long long room = static_cast<unsigned long long>(c.table_cols) << c.page_shift;
+    s.len = static_cast<uint32_t>(min(static_cast<unsigned long long>(c.kv_len[b]), min(room, 0x7FFFFFFFull)));
+  }
+  s.off = static_cast<int>(s.len) - static_cast<int>(s.rows);
+  s.tiles = (s.rows + tq - 1) / tq;
+  return s;
+}
+// Keys that row tile i sees.
+__device__ __forceinline__ uint32_t key_end(const AttnCall& c, const Seq& s, uint32_t i, uint32_t tq) {
+  if (!c.causal) return s.len;
+  const int e = s.off + static_cast<int>(min(s.rows, (i + 1) * tq));
+  return e > 0 ? static_cast<uint32_t>(e) : 0u;
+}
+// sum over i < n of floor((a i + b) / m), by Euclid's algorithm on (a, m).
+__device__ __forceinline__ unsigned long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  unsigned long long s = 0;
+  for (int guard = 0; guard < 64 && n; ++guard) {
+    if (a >= m) s += static_cast<unsigned long long>(n) * (n - 1) / 2 * (a / m), a %= m;
+    if (b >= m) s += static_cast<unsigned long long>(n) * (b / m), b %= m;
+    const unsigned long long y = static_cast<unsigned long long>(a) * n + b;
+    if (y < m) break;
+    n = static_cast<uint32_t>(y / m);
+    b = static_cast<uint32_t>(y % m);
+    const uint32_t t = m;
+    m = a;
+    a = t;
+    if (m == 0) break;
+  }
+  return s;
+}
+// Cost of the first x row tiles of a sequence (one K/V head).
+template <uint32_t KT>
+__device__ __forceinline__ unsigned long long cost_before(const AttnCall& c, const Seq& s, uint32_t x, uint32_t tq) {
+  unsigned long long w = static_cast<unsigned long long>(x) * kJobCost;
+  if (x == 0) return w;
+  if (!c.causal) return w + static_cast<unsigned long long>(x) * ((s.len + KT - 1) / KT);
+  if (x == s.tiles) w += (s.len + KT - 1) / KT, --x;  // the last tile may be short
+  // the others end at off + (i + 1) tq, those up to i0 at or before key 0
+  uint32_t i0 = 0;
+  if (s.off < 0) i0 = static_cast<uint32_t>(-s.off) / tq;
+  if (x > i0)
+    w += floor_sum(x - i0, KT, tq, static_cast<uint32_t>(s.off + static_cast<int>((i0 + 1) * tq) + static_cast<int>(KT) - 1));
+  return w;
+}
+
+// One warp: where unit u of the line lies, as (sequence, head, row tile, key tile), with a border inside a job's fixed
+// cost or near its end moved to the job's own border. (batch, 0, 0, 0) behind the last job.
+template <uint32_t KT>
+__device__ void locate(const AttnCall& c, unsigned long long u, uint32_t tq, uint32_t (&at)[4]) {
+  const uint32_t lane = threadIdx.x & 31u;
+  for (uint32_t b0 = 0; b0 < c.batch; b0 += 32) {
+    const uint32_t b = b0 + lane;
+    unsigned long long w = 0;
+    if (b < c.batch) {
+      const Seq s = load_seq(c, b, tq);
+      w = cost_before<KT>(c, s, s.tiles, tq) * c.kv_heads;
+    }
+    unsigned long long sum = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long t = __shfl_up_sync(kFullMask, sum, o);
+      if (lane >= static_cast<unsigned>(o)) sum += t;
+    }
+    const unsigned hit = __ballot_sync(kFullMask, sum > u);
+    if (hit == 0) {
+      u -= __shfl_sync(kFullMask, sum, 31);
+      continue;
+    }
+    const int src = __ffs(hit) - 1;
+    const uint32_t bb = b0 + static_cast<uint32_t>(src);
+    const unsigned long long per_seq = __shfl_sync(kFullMask, w, src);
+    unsigned long long rest = u - __shfl_sync(kFullMask, sum - w, src);
+    const Seq s = load_seq(c, bb, tq);
+    const unsigned long long per_head = per_seq / c.kv_heads;
+    uint32_t h = static_cast<uint32_t>(rest / per_head);
+    rest -= per_head * h;
+    uint32_t lo = 0, hi = s.tiles;  // cost_before(lo) <= rest < cost_before(hi)
+    while (hi - lo > 1) {
+      const uint32_t span = hi - lo, step = (span + 31) / 32, mid = lo + step * (lane + 1);
+      const bool over = mid >= hi || cost_before<KT>(c, s, mid, tq) > rest;
+      const int f = __ffs(__ballot_sync(kFullMask, over)) - 1;  // the last lane is always over
+      const uint32_t nlo = lo + step * static_cast<uint32_t>(f), nhi = min(hi, nlo + step);
+      lo = nlo;
+      hi = nhi;
+    }
+    uint32_t i = lo;
+    rest -= cost_before<KT>(c, s, i, tq);
+    const uint32_t n = (key_end(c, s, i, tq) + KT - 1) / KT;
+    uint32_t t = rest <= kJobCost ? 0u : static_cast<uint32_t>(rest) - kJobCost;
+    if (t > 0 && t + kSnap >= n) {
+      t = 0;
+      if (++i == s.tiles) {
+        i = 0;
+        if (++h == c.kv_heads) {
+          h = 0;
+          // the next sequence that has rows
+          uint32_t nb = bb + 1;
+          while (nb < c.batch && load_seq(c, nb, tq).rows == 0) ++nb;
+          at[0] = nb, at[1] = at[2] = at[3] = 0;
+          return;
+        }
+      }
+    }
+    at[0] = bb, at[1] = h, at[2] = i, at[3] = t;
+    return;
+  }
+  at[0] = c.batch, at[1] = at[2] = at[3] = 0;
+}
+
+// The pieces of jobs between two borders, one after the other.
+template <uint32_t KT>
+struct Pieces {
+  const AttnCall& c;
+  uint32_t tq, b, h, i, t;
+  uint32_t eb, eh, ei, et;
+  Seq s;
+  // the present piece
+  uint32_t t0, t1, n, keys;
+  __device__ __forceinline__ Pieces(const AttnCall& call, const Shared& sh, uint32_t tq_) : c(call), tq(tq_) {
+    b = sh.start[0], h = sh.start[1], i = sh.start[2], t = sh.start[3];
+    eb = sh.end[0], eh = sh.end[1], ei = sh.end[2], et = sh.end[3];
+    if (b < c.batch) s = load_seq(c, b, tq);
+  }
+  __device__ __forceinline__ bool next() {
+    while (true) {
+      if (b >= c.batch) return false;
+      if (s.rows == 0) {  // nothing to do for this sequence
+        if (b == eb) return false;
+        ++b;
+        h = i = t = 0;
+        if (b < c.batch) s = load_seq(c, b, tq);
+        continue;
+      }
+      break;
+    }
+    const bool last = b == eb && h == eh && i == ei;
+    if (last && t >= et) return false;
+    keys = key_end(c, s, i, tq);
+    n = (keys + KT - 1) / KT;
+    t0 = t;
+    t1 = last ? min(et, n) : n;
+    return true;
+  }
+  // Behind the present piece.
+  __device__ __forceinline__ void advance() {
+    if (b == eb && h == eh && i == ei) {
+      t = et;
+      return;
+    }
+    t = 0;
+    if (++i == s.tiles) {
+      i = 0;
+      if (++h == c.kv_heads) {
+        h = 0;
+        ++b;
+        if (b < c.batch) s = load_seq(c, b, tq);
+      }
+    }
+  }
+};
+
+// ---- the kernel -------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ CUtensorMap qmap,
+                     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using Sh = Shape<D>;
+  constexpr uint32_t KT = Sh::kKeys, ST = Sh::kStages, kChunks = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem_raw + Sh::kQBytes + ST * Sh::kStageBytes);
+  const uint32_t q_smem = smem_addr(smem_raw), kv_smem = q_smem + Sh::kQBytes;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t tq = kRows / c.group;  // tokens of a row tile
+
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < ST; ++i) bar_init(&sh.kv_full[i], 1), bar_init(&sh.kv_empty[i], 1);
+    bar_init(&sh.q_full, 1);
+    bar_init(&sh.q_empty, 1);
+    bar_init(&sh.o_empty, 8);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sh.s_full[i], 1);
+      bar_init(&sh.p_full[i], 4);
+      bar_init(&sh.pv_done[i], 1);
+      for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1);
+    }
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait_and_trigger();
+  if (warp < 2) {
+    // all of the work, and this CTA's borders (warp 0 the first, warp 1 the last)
+    unsigned long long w = 0;
+    for (uint32_t b = lane; b < c.batch; b += 32) {
+      const Seq s = load_seq(c, b, tq);
+      w += cost_before<KT>(c, s, s.tiles, tq) * c.kv_heads;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
+    const unsigned long long most = (w + kMinShare - 1) / kMinShare;
+    const uint32_t n = static_cast<uint32_t>(min(static_cast<unsigned long long>(gridDim.x), most ? most : 1ull));
+    const uint32_t x = blockIdx.x + warp;
+    uint32_t at[4] = {c.batch, 0, 0, 0};
+    if (x < n) locate<KT>(c, w / n * x + w % n * x / n, tq, at);
+    if (lane < 4) (warp ? sh.end : sh.start)[lane] = lane == 0 ? at[0] : lane == 1 ? at[1] : lane == 2 ? at[2] : at[3];
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  Pieces<KT> pc(c, sh, tq);
+  if (warp == 8) {
+    // ---- copies -------------------------------------------------------------------------------------------------
+    if (lane == 0) {
+      uint32_t g = 0, fill = 0, job = 0;
+      uint32_t issued = 0;  // loads whose completion nobody may wait for after an abort
+      const uint32_t q_bytes = kRows / c.group * c.group * 128u * kChunks;
+      auto load_kv = [&](const CUtensorMap* map, const Seq& s, uint32_t b, uint32_t h, uint32_t t, uint32_t keys, uint32_t seq) {
+        const uint32_t st = seq % ST;
+        if (seq >= ST) wait(sh, &sh.kv_empty[st], (seq / ST - 1) & 1u);
+        if (aborted(sh)) return;
+        const uint32_t base = kv_smem + st * Sh::kStageBytes, key0 = t * KT;
+        // rows behind the last visible key are left out by whole boxes
+        const uint32_t rows = min(KT, keys - key0), boxes = (rows + c.box_rows - 1) / c.box_rows;
+        stage_expect(smem_addr(&sh.kv_full[st]), boxes * c.box_rows * 128u * kChunks);
+        issued |= 1u << st;
+        for (uint32_t x = 0; x < boxes; ++x) {
+          const uint32_t key = key0 + x * c.box_rows;
+          int row = static_cast<int>(s.row0 + key), page = 0;
+          if (c.table) {
+            page = c.table[b * c.table_stride + (key >> c.page_shift)];
+            row = static_cast<int>(key & ((1u << c.page_shift) - 1u));
+          }
+          for (uint32_t ch = 0; ch < kChunks; ++ch)
+            tma_4d(base + ch * KT * 128u + x * c.box_rows * 128u, map, static_cast<int>(ch * 64), row, static_cast<int>(h), page, &sh.kv_full[st]);
+        }
+      };
+      // order of use: K(0), K(1), V(0), K(2), V(1), ...
+      uint32_t pb = 0, ph = 0, pt = 0, pkeys = 0;
+      Seq ps = {};
+      for (; pc.next() && !aborted(sh); pc.advance()) {
+        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
+          const uint32_t kslot = fill++;
+          if (g > 0) load_kv(&vmap, ps, pb, ph, pt, pkeys, fill++);
+          if (t == pc.t0) {
+            if (job > 0) wait(sh, &sh.q_empty, (job - 1) & 1u);
+            if (aborted(sh)) break;
+            stage_expect(smem_addr(&sh.q_full), q_bytes);
+            for (uint32_t ch = 0; ch < kChunks; ++ch)
+              tma_3d(q_smem + ch * kRows * 128u, &qmap, static_cast<int>(ch * 64), static_cast<int>(pc.h * c.group),
+                     static_cast<int>(pc.s.row0 + pc.i * tq), &sh.q_full);
+            ++job;
+          }
+          load_kv(&kmap, pc.s, pc.b, pc.h, t, pc.keys, kslot);
+          ps = pc.s, pb = pc.b, ph = pc.h, pt = t, pkeys = pc.keys;
+        }
+      }
+      if (g > 0 && !aborted(sh)) load_kv(&vmap, ps, pb, ph, pt, pkeys, fill++);
+      if (aborted(sh)) {
+        // no copy may land in shared memory that another CTA owns by then: one more bounded wait for each
+        for (uint32_t st = 0; st < ST; ++st)
+          if (issued >> st & 1u) {
+            stage_wait(smem_addr(&sh.kv_full[st]), 0);
+            stage_wait(smem_addr(&sh.kv_full[st]), 1);
+          }
+        if (job) {
+          stage_wait(smem_addr(&sh.q_full), 0);
+          stage_wait(smem_addr(&sh.q_full), 1);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---- matrix products ----------------------------------------------------------------------------------------
+    constexpr uint32_t idesc_s = instr_desc<T>(kRows, KT, false), idesc_o = instr_desc<T>(kRows, D, true);
+    uint32_t g = 0, fill = 0, job = 0;
+    uint32_t prev_first = 0, prev_valid = 0, prev_job = 0;  // of tile g - 1
+    auto pv = [&](uint32_t gt, uint32_t slot, bool first, uint32_t valid, uint32_t jobno) {
+      const uint32_t st = slot % ST, buf = gt & 1u, base = kv_smem + st * Sh::kStageBytes;
+      wait(sh, &sh.kv_full[st], (slot / ST) & 1u);
+      if (valid < KT) {
+        // V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: clear them
+        for (uint32_t x = lane; x < (KT - valid) * 8u * kChunks; x += 32) {
+          const uint32_t ch = x / ((KT - valid) * 8u), y = x - ch * ((KT - valid) * 8u);
+          const uint32_t at = base + ch * KT * 128u + valid * 128u + y * 16u;
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if (first && jobno > 0) wait(sh, &sh.o_empty, (jobno - 1) & 1u);
+      wait(sh, &sh.p_full[buf], (gt >> 1) & 1u);
+      tc_after();
+      if (lane == 0 && !aborted(sh)) {
+        const uint64_t vd = smem_desc(base, KT * 128u);
+#pragma unroll
+        for (uint32_t k = 0; k < KT / 16; ++k)
+          mma_ts(tmem + kTmemO, tmem + buf * 128u + k * 8u, vd + k * (2048u >> 4), idesc_o, !(first && k == 0));
+        tc_commit(&sh.kv_empty[st]);
+        tc_commit(&sh.pv_done[buf]);
+      }
+      __syncwarp();
+    };
+    uint32_t vslot = 0;
+    for (; pc.next() && !aborted(sh); pc.advance()) {
+      for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
+        const uint32_t kslot = fill++, buf = g & 1u, st = kslot % ST;
+        if (g > 0) vslot = fill++;
+        if (t == pc.t0) wait(sh, &sh.q_full, job & 1u);
+        wait(sh, &sh.kv_full[st], (kslot / ST) & 1u);
+        tc_after();
+        if (lane == 0 && !aborted(sh)) {
+          const uint64_t qd = smem_desc(q_smem, 16), kd = smem_desc(kv_smem + st * Sh::kStageBytes, 16);
+#pragma unroll
+          for (uint32_t k = 0; k < D / 16; ++k)
+            mma_ss(tmem + buf * 128u, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u, kd + ((k >> 2) * KT * 128u + (k & 3u) * 32u) / 16u,
+                   idesc_s, k > 0);
+          tc_commit(&sh.kv_empty[st]);
+          tc_commit(&sh.s_full[buf]);
+          if (t + 1 == pc.t1) tc_commit(&sh.q_empty);
+        }
+        __syncwarp();
+        if (g > 0) pv(g - 1, vslot, prev_first != 0, prev_valid, prev_job);
+        prev_first = t == pc.t0;
+        prev_valid = min(KT, pc.keys - t * KT);
+        prev_job = job;
+      }
+      if (pc.t1 > pc.t0) ++job;
+    }
+    if (g > 0 && !aborted(sh)) pv(g - 1, fill++, prev_first != 0, prev_valid, prev_job);
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    Pieces<KT> pc(c, sh, tq);
+    // ---- softmax, and the outputs -------------------------------------------------------------------------------
+    const uint32_t wg = warp >> 2, quad = warp & 3u, row = quad * 32u + lane;
+    const uint32_t lane_base = (quad * 32u) << 16;
+    const uint32_t my_tok = row / c.group, my_head = row - my_tok * c.group;
+    uint32_t g = 0;
+    if (threadIdx.x == 0) c.meta[8u * blockIdx.x] = c.meta[8u * blockIdx.x + 1] = 0;
+    for (; pc.next(); pc.advance()) {
+      const uint32_t tok0 = pc.i * tq, toks = min(tq, pc.s.rows - tok0), rows = toks * c.group;
+      const bool busy = quad * 32u < rows;  // warps without a row only keep step
+      // keys that this row sees
+      uint32_t limit = pc.keys;
+      if (c.causal) limit = static_cast<uint32_t>(max(0, min(static_cast<int>(pc.keys), pc.s.off + static_cast<int>(tok0 + my_tok) + 1)));
+      const uint32_t all_see = c.causal ? static_cast<uint32_t>(max(0, pc.s.off + static_cast<int>(tok0) + 1)) : pc.keys;
+      float m = -INFINITY, l = 0.0f;  // the reference that l is relative to
+      for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
+        const uint32_t buf = g & 1u;
+        if (buf != wg) continue;
+        wait(sh, &sh.s_full[buf], (g >> 1) & 1u);
+        tc_after();
+        if (busy) {
+          float s[KT / 32][32];
+#pragma unroll
+          for (uint32_t x = 0; x < KT / 32; ++x) tc_ld32(tmem + lane_base + buf * 128u + x * 32u, s[x]);
+          tc_wait_ld(s);
+          const uint32_t key0 = t * KT;
+          if (key0 + KT > min(all_see, pc.keys)) {
+            const uint32_t left = limit > key0 ? limit - key0 : 0u;
+#pragma unroll
+            for (uint32_t x = 0; x < KT; ++x)
+              if (x >= left) s[x / 32][x % 32] = -INFINITY;
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (uint32_t x = 0; x < KT; x += 2) mx = max3f(mx, s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
+          if (row >= rows) mx = -INFINITY;  // no query row: what stands there has no say
+          float ref = -INFINITY;
+          if (t > pc.t0) {
+            wait(sh, &sh.m_full[buf ^ 1u][quad], ((g - 1) >> 1) & 1u);
+            ref = sh.m[buf ^ 1u][row];
+          }
+          // the reference follows where it has fallen too far behind
+          const float grown = __fmul_rn(mx - ref, c.scale_log2);
+          const bool follow = grown > kLazy;  // also from -inf; false for -inf against -inf (NaN)
+          const float next_ref = follow ? mx : ref;
+          if (__any_sync(kFullMask, follow && ref != -INFINITY)) {
+            wait(sh, &sh.pv_done[buf ^ 1u], ((g - 1) >> 1) & 1u);
+            tc_after();
+            const float f = follow && ref != -INFINITY ? ex2_approx(-grown) : 1.0f;
+#pragma unroll 1
+            for (uint32_t x = 0; x < D / 32; ++x) {
+              float o[32];
+              tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
+              tc_wait_ld(o);
+              uint32_t r[32];
+#pragma unroll
+              for (int y = 0; y < 32; ++y) r[y] = __float_as_uint(__fmul_rn(o[y], f));
+              tc_st32(tmem + lane_base + kTmemO + x * 32u, r);
+            }
+            tc_wait_st();
+          }
+          sh.m[buf][row] = next_ref;
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.m_full[buf][quad]);
+          // p = 2^(c s - c ref); a row that has seen nothing yet has s = -inf everywhere, and 0 does for its reference
+          const float mc = next_ref == -INFINITY ? 0.0f : __fmul_rn(next_ref, c.scale_log2);
+          const float2 c2 = make_float2(c.scale_log2, c.scale_log2), m2 = make_float2(-mc, -mc);
+          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (uint32_t x = 0; x < KT / 64; ++x) {
+            uint32_t r[32];
+#pragma unroll
+            for (uint32_t y = 0; y < 32; ++y) {
+              const uint32_t at = x * 64 + 2 * y;
+              float2 v = __ffma2_rn(make_float2(s[at / 32][at % 32], s[at / 32][at % 32 + 1]), c2, m2);
+              v.x = ex2_approx(v.x);
+              v.y = ex2_approx(v.y);
+              sum = __fadd2_rn(sum, v);
+              r[y] = pack2<T>(v.x, v.y);
+            }
+            tc_st32(tmem + lane_base + buf * 128u + x * 32u, r);
+          }
+          if (next_ref != m) {
+            if (m != -INFINITY) l = __fmul_rn(l, ex2_approx(__fmul_rn(m - next_ref, c.scale_log2)));
+            m = next_ref;
+          }
+          l += sum.x + sum.y;
+          tc_wait_st();
+        } else {
+          if (lane == 0) bar_arrive(&sh.m_full[buf][quad]);
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh.p_full[buf]);
+      }
+      // the two groups' denominators over one reference, the last tile's
+      const bool any = pc.t1 > pc.t0;
+      float ref = m;
+      if (any && ((g - 1) & 1u) != wg) {
+        wait(sh, &sh.m_full[(g - 1) & 1u][quad], ((g - 1) >> 1) & 1u);
+        ref = sh.m[(g - 1) & 1u][row];
+        if (!busy) ref = -INFINITY;
+        if (m != -INFINITY && ref != m) l = __fmul_rn(l, ex2_approx(__fmul_rn(m - ref, c.scale_log2)));
+      }
+      sh.l[wg][row] = l;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const float total = sh.l[0][row] + sh.l[1][row];
+      const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
+      if (any) {
+        wait(sh, &sh.pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u);
+        tc_after();
+      }
+      const bool mine = row < rows && !aborted(sh);
+      const uint64_t token = pc.s.row0 + tok0 + my_tok;
+      const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+      constexpr uint32_t kHalf = D / 2;  // columns of a group
+      if (busy) {
+        float* piece = nullptr;
+        if (!whole) piece = c.part + (2ull * blockIdx.x + (pc.t0 == 0 ? 1u : 0u)) * AttnPieceFloats(D);
+#pragma unroll 1
+        for (uint32_t x = 0; x < kHalf / 32; ++x) {
+          const uint32_t col = wg * kHalf + x * 32u;
+          float o[32];
+          if (any) {
+            tc_ld32(tmem + lane_base + kTmemO + col, o);
+            tc_wait_ld(o);
+          }
+          if (!any || total == 0.0f) {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+          }
+          if (!mine) continue;
+          if (whole) {
+            T* to = static_cast<T*>(c.out) + token * c.out_row + (pc.h * c.group + my_head) * c.out_head;
+#pragma unroll
+            for (uint32_t y = 0; y < 32; y += 8)
+              if (col + y < c.dim) {
+                uint4 u;
+                u.x = pack2<T>(__fmul_rn(o[y], inv), __fmul_rn(o[y + 1], inv));
+                u.y = pack2<T>(__fmul_rn(o[y + 2], inv), __fmul_rn(o[y + 3], inv));
+                u.z = pack2<T>(__fmul_rn(o[y + 4], inv), __fmul_rn(o[y + 5], inv));
+                u.w = pack2<T>(__fmul_rn(o[y + 6], inv), __fmul_rn(o[y + 7], inv));
+                *reinterpret_cast<uint4*>(to + col + y) = u;
+              }
+          } else {
+            // [column / 4][row] quads, so that a warp's rows lie side by side
+#pragma unroll
+            for (uint32_t y = 0; y < 32; y += 4)
+              *reinterpret_cast<float4*>(piece + ((col + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+          }
+        }
+        if (mine && wg == 0) {
+          if (whole) {
+            if (c.lse) {
+              const float lse = total == 0.0f ? -INFINITY
+                                              : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total)), 0.69314718055994531f);
+              c.lse[token * (c.kv_heads * c.group) + pc.h * c.group + my_head] = lse;
+            }
+          } else {
+            piece[D * kRows + row] = ref;
+            piece[(D + 1) * kRows + row] = total;
+          }
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (any && lane == 0) bar_arrive(&sh.o_empty);
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // before sh.l is written again
+      if (threadIdx.x == 0 && !whole) {
+        // what the join needs: a piece that opens a split job says which one, every other one whether it ends it
+        uint32_t* to = c.meta + 8u * blockIdx.x;
+        if (pc.t0 == 0) to[1] = 1u, to[2] = pc.b, to[3] = pc.h, to[4] = pc.i;
+        else to[0] = pc.t1 == pc.n ? 2u : 1u;
+      }
+    }
+  }
+
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+
+// ---- joining the pieces of split jobs -----------------------------------------------------------------------------
+// out = sum_p 2^(c (r_p - R)) O_p / sum_p 2^(c (r_p - R)) l_p over a job's pieces p, R the largest of their references.
+// blockIdx.x: the split job, counted over the CTAs that opened one; blockIdx.y: 32 rows and a share of the columns. Few
+// pieces (a prompt's jobs are cut once): a warp sums a column quad over all of them; many (one token over a long cache
+// is cut by every CTA): the warps share the pieces and meet in shared memory. The order of the sums is fixed.
+constexpr uint32_t kJoinWarps = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnCall c, const uint32_t ctas) {
+  __shared__ uint32_t opens[(kMaxCtas + 31) / 32], ends[(kMaxCtas + 31) / 32];
+  __shared__ float weight[kMaxCtas + 1][32];
+  __shared__ float4 red[kJoinWarps][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  pdl_wait_and_trigger();
+  if (warp < (kMaxCtas + 31) / 32) {
+    const uint32_t x = warp * 32u + lane;
+    const uint32_t f0 = x < ctas ? c.meta[8u * x] : 0u, f1 = x < ctas ? c.meta[8u * x + 1] : 0u;
+    const uint32_t o = __ballot_sync(kFullMask, f1 == 1u), e = __ballot_sync(kFullMask, f0 == 2u);
+    if (lane == 0) opens[warp] = o, ends[warp] = e;
+  }
+  __syncthreads();
+  uint32_t k = blockIdx.x, first = kMaxCtas;
+  for (uint32_t w = 0; w < (kMaxCtas + 31) / 32; ++w) {
+    const uint32_t n = __popc(opens[w]);
+    if (k < n) {
+      uint32_t v = opens[w];
+      for (; k; --k) v &= v - 1;
+      first = w * 32u + __ffs(v) - 1;
+      break;
+    }
+    k -= n;
+  }
+  if (first >= ctas) return;
+  uint32_t last = first;
+  for (uint32_t w = (first + 1) / 32; w < (kMaxCtas + 31) / 32; ++w) {
+    uint32_t v = ends[w];
+    if (w == (first + 1) / 32) v &= ~0u << ((first + 1) & 31u);
+    if (v) {
+      last = w * 32u + __ffs(v) - 1;
+      break;
+    }
+  }
+  const uint32_t pieces = last - first + 1;
+  const uint32_t* job = c.meta + 8u * first;
+  const uint32_t h = job[3], tq = kRows / c.group, tok0 = job[4] * tq;
+  const Seq s = load_seq(c, job[2], tq);
+  const uint32_t rows = min(tq, s.rows - tok0) * c.group;
+  const uint32_t row = (blockIdx.y & 3u) * 32u + lane;
+  if ((blockIdx.y & 3u) * 32u >= rows) return;
+  // piece 0 opened the job, the others are what the CTAs behind began with
+  auto piece = [&](uint32_t p) { return c.part + (2ull * (first + p) + (p == 0 ? 1u : 0u)) * AttnPieceFloats(D); };
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps) weight[p][lane] = row < rows ? piece(p)[D * kRows + row] : -INFINITY;
+  __syncthreads();
+  float top = -INFINITY;
+  for (uint32_t p = 0; p < pieces; ++p) top = fmaxf(top, weight[p][lane]);
+  __syncthreads();
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
+    const float r = weight[p][lane];
+    weight[p][lane] = r == -INFINITY ? 0.0f : ex2_approx(__fmul_rn(r - top, c.scale_log2));
+  }
+  __syncthreads();
+  float total = 0.0f;
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps)
+    if (row < rows) {
+      const float w = weight[p][lane];
+      if (w != 0.0f) total = __fmaf_rn(w, piece(p)[(D + 1) * kRows + row], total);
+    }
+  red[warp][lane].x = total;
+  __syncthreads();
+  total = 0.0f;
+#pragma unroll
+  for (uint32_t w = 0; w < kJoinWarps; ++w) total += red[w][lane].x;
+  __syncthreads();
+  const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+  const uint64_t token = s.row0 + tok0 + row / c.group;
+  const uint32_t head = h * c.group + row % c.group;
+  T* out = static_cast<T*>(c.out) + token * c.out_row + head * c.out_head;
+  if (c.lse && blockIdx.y < 4 && warp == 0 && row < rows)
+    c.lse[token * (c.kv_heads * c.group) + head] =
+        total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total)), 0.69314718055994531f);
+  const bool shared = pieces > 4;
+  const uint32_t p0 = shared ? warp : 0u, pstep = shared ? kJoinWarps : 1u;
+  const uint32_t parts = gridDim.y >> 2, quads = D / 4 / parts, q0 = (blockIdx.y >> 2) * quads;
+  for (uint32_t q = q0 + (shared ? 0u : warp); q < q0 + quads; q += shared ? 1u : kJoinWarps) {
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (row < rows) {
+#pragma unroll 4
+      for (uint32_t p = p0; p < pieces; p += pstep) {
+        const float4 v = *reinterpret_cast<const float4*>(piece(p) + (q * kRows + row) * 4);
+        const float w = weight[p][lane];
+        if (w != 0.0f) {  // a piece that saw nothing says nothing
+          sum.x = __fmaf_rn(w, v.x, sum.x);
+          sum.y = __fmaf_rn(w, v.y, sum.y);
+          sum.z = __fmaf_rn(w, v.z, sum.z);
+          sum.w = __fmaf_rn(w, v.w, sum.w);
+        }
+      }
+    }
+    if (shared) {
+      red[warp][lane] = sum;
+      __syncthreads();
+      sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (warp == 0) {
+#pragma unroll
+        for (uint32_t w = 0; w < kJoinWarps; ++w) sum.x += red[w][lane].x, sum.y += red[w][lane].y, sum.z += red[w][lane].z, sum.w += red[w][lane].w;
+      }
+      __syncthreads();
+    }
+    if (row < rows && q * 4 < c.dim && (!shared || warp == 0)) {
+      uint2 u;
+      u.x = pack2<T>(__fmul_rn(sum.x, inv), __fmul_rn(sum.y, inv));
+      u.y = pack2<T>(__fmul_rn(sum.z, inv), __fmul_rn(sum.w, inv));
+      *reinterpret_cast<uint2*>(out + q * 4) = u;
+    }
+  }
+}
+
+// ---- launch -----------------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn Encoder() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// A map over 16-bit elements with 128-byte swizzle; dims[0] is contiguous, strides in elements. The stride of an axis
+// with one entry is never used, but has to pass the encoder's checks.
+cudaError_t MakeMap(CUtensorMap* map, int dtype, const void* base, uint32_t rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  const EncodeFn encode = Encoder();
+  if (!encode) return cudaErrorNotSupported;
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4], es[4] = {1, 1, 1, 1};
+  for (uint32_t i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
+  for (uint32_t i = 1; i < rank; ++i) st[i - 1] = dims[i] == 1 ? 16 * ((dims[0] * 2 + 15) / 16) : strides[i] * 2;
+  const CUresult r = encode(map, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), d,
+                            st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+constexpr uint64_t kMetaBytes = 8192;
+static_assert(kMetaBytes >= kMaxCtas * 32, "eight words for each CTA");
+constexpr uint32_t PadDim(uint32_t dim) { return dim <= 64 ? 64u : dim <= 128 ? 128u : 256u; }
+
+template <typename T, int D>
+cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
+  AttnCall c{};
+  c.cu = a.cu;
+  c.kv_len = a.kv_len;
+  c.table = a.table;
+  c.table_stride = a.table_stride;
+  c.table_cols = a.table_cols;
+  c.page_shift = a.page_shift;
+  c.batch = a.batch;
+  c.tokens = a.tokens;
+  c.kv_heads = a.kv_heads;
+  c.group = a.q_heads / a.kv_heads;
+  c.dim = a.dim;
+  c.causal = a.causal;
+  c.scale_log2 = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
+  c.out = a.out;
+  c.out_row = a.out_row;
+  c.out_head = a.out_head;
+  c.lse = a.lse;
+  c.meta = static_cast<uint32_t*>(a.workspace);
+  c.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kMetaBytes);
+  const uint32_t tq = kRows / c.group;
+  c.box_rows = a.table && (1u << a.page_shift) < 64u ? 1u << a.page_shift : 64u;
+
+  CUtensorMap qm, km, vm;
+  const uint64_t qd[3] = {a.dim, a.q_heads, a.tokens}, qs[3] = {1, a.q_head, a.q_row};
+  const uint32_t qb[3] = {64, c.group, tq};
+  cudaError_t e = MakeMap(&qm, a.dtype, a.q, 3, qd, qs, qb);
+  if (e != cudaSuccess) return e;
+  const uint64_t rows = a.table ? uint64_t{1} << a.page_shift : a.tokens, pages = a.table ? a.pages : 1;
+  const uint64_t kd[4] = {a.dim, rows, a.kv_heads, pages};
+  const uint64_t ks[4] = {1, a.k_row, a.k_head, a.k_page}, vs[4] = {1, a.v_row, a.v_head, a.v_page};
+  const uint32_t kb[4] = {64, c.box_rows, 1, 1};
+  e = MakeMap(&km, a.dtype, a.k, 4, kd, ks, kb);
+  if (e == cudaSuccess) e = MakeMap(&vm, a.dtype, a.v, 4, kd, vs, kb);
+  if (e != cudaSuccess) return e;
+
+  int dev = 0, sms = 0;
+  e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes<D>));
+  if (e != cudaSuccess) return e;
+  const uint64_t most_keys = a.table ? static_cast<uint64_t>(a.table_cols) << a.page_shift : a.tokens;
+  const uint64_t jobs = (static_cast<uint64_t>(a.tokens) / tq + a.batch) * a.kv_heads;  // at most
+  const uint64_t tiles = (most_keys + Shape<D>::kKeys - 1) / Shape<D>::kKeys;
+  uint64_t ctas = (jobs * (tiles + kJobCost) + kMinShare - 1) / kMinShare;
+  if (ctas > static_cast<uint64_t>(sms)) ctas = static_cast<uint64_t>(sms);
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
+  if (ctas < 1) ctas = 1;
+  e = LaunchKernel(attention_kernel<T, D>, static_cast<unsigned>(ctas), kThreads, kSmemBytes<D>, s, c, qm, km, vm);
+  // jobs of one tile are never split
+  if (e != cudaSuccess || tiles <= 1 || ctas == 1) return e;
+  const uint32_t x = static_cast<uint32_t>(jobs < ctas ? jobs : ctas);
+  uint32_t parts = 1;
+  while (parts < 16 && x * 4 * parts * 2 <= 148 * 8) parts *= 2;
+  return LaunchKernel(attention_join_kernel<T, D>, dim3(x, 4 * parts), kJoinWarps * 32, 0, s, c, static_cast<uint32_t>(ctas));
+}
+
+template <typename T>
+cudaError_t LaunchDim(const AttnArgs& a, cudaStream_t s) {
+  switch (PadDim(a.dim)) {
+    case 64: return Launch<T, 64>(a, s);
+    case 128: return Launch<T, 128>(a, s);
+    default: return Launch<T, 256>(a, s);
+  }
+}
+
+}  // namespace
+
+uint64_t AttentionWorkspaceBytes(uint32_t dim) { return kMetaBytes + 2ull * kMaxCtas * AttnPieceFloats(PadDim(dim)) * 4; }
+
+cudaError_t LaunchAttention(const AttnArgs& a, cudaStream_t s) {
+  return a.dtype == kBF16 ? LaunchDim<bf16>(a, s) : LaunchDim<f16>(a, s);
+}
+
+cudaError_t ReadAttentionTimeouts(unsigned int* out) { return cudaMemcpyFromSymbol(out, g_attn_timeouts, sizeof(unsigned int)); }
+
+}  // namespace halo_b200

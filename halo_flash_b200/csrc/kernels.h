@@ -365,6 +365,61 @@ struct MoeCombineArgs {
 };
 cudaError_t LaunchMoeCombine(const MoeCombineArgs& a, cudaStream_t s);
 
+// ---- paged K/V cache and attention ---------------------------------------------------------------
+struct PlanArgs {
+  int32_t* table;  // [batch][table_stride], table_cols of each row in use
+  uint64_t table_stride;
+  uint32_t table_cols;
+  const uint32_t* past;
+  const uint32_t* fresh;
+  const int32_t* free_pages;
+  uint32_t n_free, page_shift, batch, tokens;
+  int64_t* slot;     // [tokens]
+  uint32_t* pos;     // [tokens] or null
+  uint32_t* cu;      // [batch + 1] or null
+  uint32_t* kv_len;  // [batch] or null
+  uint32_t* status;  // [3] or null
+};
+constexpr uint32_t kMaxPlanBatch = 16384;
+cudaError_t LaunchPagedPlan(const PlanArgs& a, cudaStream_t s);
+
+// Rows of K and V [tokens][heads][dim] to the rows of a paged cache that their slots name.
+struct StoreArgs {
+  const void* src[2];  // k, v
+  void* dst[2];
+  int src_dtype, dst_dtype;
+  uint64_t src_row[2], src_head[2];             // element strides
+  uint64_t page_stride, row_stride, head_stride;  // of both caches, in elements
+  const int64_t* slot;
+  uint32_t tokens, heads, dim, page_shift, pages;
+  int vec;
+};
+cudaError_t LaunchPagedStore(const StoreArgs& a, cudaStream_t s);
+
+struct AttnArgs {
+  const void* q;
+  uint64_t q_row, q_head;
+  const void *k, *v;
+  uint64_t k_row, k_head, k_page, v_row, v_head, v_page;  // element strides; pages only in the paged form
+  uint32_t pages, page_shift;
+  int dtype;
+  const int32_t* table;  // null: packed
+  uint64_t table_stride;
+  uint32_t table_cols;
+  const uint32_t* kv_len;
+  const uint32_t* cu;
+  uint32_t batch, tokens, q_heads, kv_heads, dim;
+  float scale;
+  int causal;
+  void* out;
+  uint64_t out_row, out_head;
+  float* lse;
+  void* workspace;
+};
+uint64_t AttentionWorkspaceBytes(uint32_t dim);
+cudaError_t LaunchAttention(const AttnArgs& a, cudaStream_t s);
+cudaError_t ReadAttentionTimeouts(unsigned int* out);
+
 
 }  // namespace halo_b200
 

@@ -314,3 +314,136 @@ def moe_combine(yp, pos, mw, out, *, sx=None, sg=None):
     lib().call("moe_combine_ex", _stream(), _p(yp), _code(yp), _p(pos), _p(mw), _p(sx), _code(sx) if sx is not None else F32,
                _p(sg), _p(out), _code(out), k, n, tokens)
     return out
+
+
+# ---- paged K/V cache and attention ----------------------------------------------------------------
+_INT = (torch.int32, torch.uint32)
+
+
+def _here(*tensors):
+    """The kernels run on the current device's current stream: every tensor must live there."""
+    for t in tensors:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _rows(t, name, dtypes, rank=3):
+    """A CUDA tensor of `rank` axes whose last one is contiguous; the other strides are free."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name}: expected a CUDA tensor (halo_flash_b200 has no CPU path)")
+    if t.dim() != rank:
+        raise ValueError(f"{name}: expected {rank} axes, got shape {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {dtypes}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    return t
+
+
+def _strides(t, *axes):
+    """Strides in elements; an axis of one entry is never stepped along, whatever torch says its stride is."""
+    return [t.stride(a) if t.shape[a] > 1 else 0 for a in axes]
+
+
+def _caches(k_cache, v_cache, dtypes):
+    _rows(k_cache, "k_cache", dtypes, 4), _rows(v_cache, "v_cache", (k_cache.dtype,), 4)
+    if k_cache.shape != v_cache.shape or _strides(k_cache, 0, 1, 2) != _strides(v_cache, 0, 1, 2):
+        raise ValueError("k_cache and v_cache must have the same shape and strides")
+    return k_cache.shape
+
+
+def _table(table):
+    _rows(table, "table", _INT, 2)
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError("table: rows overlap")
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1]
+
+
+def _vector(t, name, dtypes, n):
+    _chk(t, name, dtypes)
+    if t is not None and t.numel() != n:
+        raise ValueError(f"{name}: expected {n} entries, got {t.numel()}")
+    return t
+
+
+def paged_plan(table, past, fresh, free_pages, page_size, slot, *, pos=None, cu=None, kv_len=None, status=None):
+    """The plan of one step of a paged cache: request r holds past[r] tokens in the pages of table[r] and gets fresh[r]
+    more. The pages it needs come from free_pages in order and go into its table row; slot (int64) gets every new
+    token's page * page_size + offset (-1: refused, or behind the last new token), pos its position, cu [B + 1] the
+    prefix sum of fresh, kv_len past + fresh, status [pages taken, requests refused, new tokens]. A request that the
+    table row or the free list cannot hold is refused: no pages, slots -1, kv_len = past."""
+    stride, cols = _table(table)
+    batch = table.shape[0]
+    _vector(past, "past", _INT, batch), _vector(fresh, "fresh", _INT, batch), _chk(free_pages, "free_pages", _INT)
+    _chk(slot, "slot", (torch.int64,)), _vector(pos, "pos", _INT, slot.numel()), _vector(cu, "cu", _INT, batch + 1)
+    _vector(kv_len, "kv_len", _INT, batch), _vector(status, "status", _INT, 3)
+    _here(table, past, fresh, free_pages, slot, pos, cu, kv_len, status)
+    lib().call("paged_plan", _stream(), _p(table), stride, cols, _p(past), _p(fresh), _p(free_pages), free_pages.numel(),
+               page_size, _p(slot), _p(pos), _p(cu), _p(kv_len), _p(status), batch, slot.numel())
+    return slot
+
+
+def paged_store(k, v, k_cache, v_cache, slot):
+    """Rows k, v [T, heads, d] to the rows of the caches [pages, page_size, heads, d] that slot (int64 [T]) names;
+    slots outside the cache are skipped, and no two of a call may be equal. The caches may be views of any strides."""
+    pages, page_size, heads, d = _caches(k_cache, v_cache, _ACT)
+    _rows(k, "k", _ACT), _rows(v, "v", (k.dtype,)), _vector(slot, "slot", (torch.int64,), k.shape[0])
+    if k.shape != v.shape or tuple(k.shape[1:]) != (heads, d):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit caches of {heads} heads of {d}")
+    _here(k, v, k_cache, v_cache, slot)
+    lib().call("paged_store", _stream(), _p(k), *_strides(k, 0, 1), _p(v), *_strides(v, 0, 1), _code(k), _p(k_cache),
+               _p(v_cache), _code(k_cache), *_strides(k_cache, 0, 1, 2), pages, page_size, _p(slot), heads, d, k.shape[0])
+
+
+def attention_workspace(d, device=None):
+    """The workspace of the attention calls for head size d. Calls that may overlap on the GPU need one each; None in
+    the calls below takes a fresh one from torch's allocator."""
+    return torch.empty(lib().cdll.halo_b200_attention_workspace(d), dtype=torch.uint8, device=device or "cuda")
+
+
+def _attention(q, out, cu, lse, workspace, scale):
+    _rows(q, "q", (torch.float16, torch.bfloat16)), _rows(out, "out", (q.dtype,)), _chk(cu, "cu", _INT)
+    if out.shape != q.shape:
+        raise ValueError(f"out {tuple(out.shape)} must have the shape of q {tuple(q.shape)}")
+    if cu.numel() < 1:
+        raise ValueError("cu: expected batch + 1 entries")
+    _vector(lse, "lse", (torch.float32,), q.shape[0] * q.shape[1])
+    if workspace is None:
+        workspace = attention_workspace(q.shape[2], q.device)
+    _chk(workspace, "workspace")
+    return workspace, workspace.numel() * workspace.element_size(), q.shape[2] ** -0.5 if scale is None else scale
+
+
+def attention_packed(q, k, v, cu, out, *, scale=None, causal=True, lse=None, workspace=None):
+    """Attention of packed sequences: rows cu[b] .. cu[b + 1] of q, out [T, Hq, d] and k, v [T, Hk, d] are sequence b.
+    Query head h reads K/V head h // (Hq // Hk). scale defaults to d ** -0.5; lse (optional, fp32 [T, Hq]) gets the
+    logarithm of each softmax denominator. Rows behind cu[-1] are left as they are."""
+    ws, ws_bytes, scale = _attention(q, out, cu, lse, workspace, scale)
+    _rows(k, "k", (q.dtype,)), _rows(v, "v", (q.dtype,))
+    tokens, hq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != d:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    _here(q, k, v, cu, out, lse, ws)
+    lib().call("attention_packed", _stream(), _p(q), *_strides(q, 0, 1), _p(k), *_strides(k, 0, 1), _p(v), *_strides(v, 0, 1),
+               _p(out), *_strides(out, 0, 1), _code(q), _p(cu), cu.numel() - 1, tokens, hq, k.shape[1], d, scale, int(causal),
+               _p(lse), _p(ws), ws_bytes)
+    return out
+
+
+def attention_paged(q, k_cache, v_cache, table, kv_len, cu, out, *, scale=None, causal=True, lse=None, workspace=None):
+    """Attention of new tokens over a paged cache that already holds them: rows cu[b] .. cu[b + 1] of q, out [T, Hq, d]
+    are the newest of sequence b's kv_len[b] tokens, whose K and V stand in the pages table[b] of the caches
+    [pages, page_size, Hk, d]. One row for each sequence is a decode step, more are a prompt's chunk, in any mixture."""
+    ws, ws_bytes, scale = _attention(q, out, cu, lse, workspace, scale)
+    pages, page_size, heads, d = _caches(k_cache, v_cache, (q.dtype,))
+    stride, cols = _table(table)
+    batch = cu.numel() - 1
+    _vector(kv_len, "kv_len", _INT, batch)
+    tokens, hq, dq = q.shape
+    if dq != d or table.shape[0] != batch:
+        raise ValueError(f"q {tuple(q.shape)}, table {tuple(table.shape)} and cu do not fit caches {tuple(k_cache.shape)}")
+    _here(q, k_cache, v_cache, table, kv_len, cu, out, lse, ws)
+    lib().call("attention_paged", _stream(), _p(q), *_strides(q, 0, 1), _p(k_cache), _p(v_cache), *_strides(k_cache, 0, 1, 2),
+               pages, page_size, _p(table), stride, cols, _p(kv_len), _p(out), *_strides(out, 0, 1), _code(q), _p(cu), batch,
+               tokens, hq, heads, d, scale, int(causal), _p(lse), _p(ws), ws_bytes)
+    return out

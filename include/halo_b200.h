@@ -499,6 +499,77 @@ int halo_b200_f16_rows(halo_b200_stream stream, const float* x, uint16_t* y, uin
 int halo_b200_scale_silu(halo_b200_stream stream, const float* x, void* y, int y_dtype, float scale, uint32_t n,
                          char* err, size_t errlen);
 
+/* ---- paged K/V cache, and attention over it and over packed prompts ------------------------------- */
+
+/* No counterpart in the reference's kernels: the plan of one step of a paged K/V cache, built on the device from
+ * lengths alone. Pages hold page_size tokens (a power of two, 8 .. 256). Request r holds past[r] tokens in the pages
+ * table[r * table_stride + 0 ..] and gets fresh[r] more; the pages it needs beyond ceil(past / page_size) are taken
+ * from free_pages in request order and written to its table row (entries beyond those are not touched). Outputs:
+ *   slot[t]   page * page_size + offset of the t-th new token (new tokens of all requests, one request after the other)
+ *   pos[t]    its position, past[r] + i: what halo_b200_rope_table_ex reads as params (pstride 1); optional
+ *   cu        [batch + 1] prefix sum of fresh; optional
+ *   kv_len[r] past[r] + fresh[r]: the past of the next step; optional
+ *   status    [3]: pages taken, requests refused, new tokens; optional
+ * A request that needs more than table_cols pages, or whose pages would pass the end of the free list, is refused: it
+ * takes no page, its slots are -1 and its kv_len stays past[r]. Requests are served in order: once the list cannot
+ * serve one, it serves none behind it that needs a page. slot and pos have `tokens` entries: those behind the last
+ * new token get -1 and 0, new tokens beyond them get none. batch <= 16384, n_free < 2^31, lengths < 2^31. */
+int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table_stride, uint32_t table_cols,
+                         const uint32_t* past, const uint32_t* fresh, const int32_t* free_pages, uint32_t n_free,
+                         uint32_t page_size, int64_t* slot, uint32_t* pos, uint32_t* cu, uint32_t* kv_len,
+                         uint32_t* status, uint32_t batch, uint32_t tokens, char* err, size_t errlen);
+
+/* No counterpart in the reference's kernels (halo_copy_at appends one row, src/kernels/core.hip:341-350): rows k, v
+ * [tokens][heads][dim] of `dtype` to the cache rows that slot names. Element (page, row, head, i) of either cache is
+ * at page * page_stride + row * row_stride + head * head_stride + i. A slot that is negative or not below
+ * pages * page_size is skipped. The slots of a call must differ: of two rows with the same slot either may remain.
+ * (dtype, cache_dtype) in (f32, f32|f16|bf16), (f16, f16|bf16), (bf16, bf16|f16). All strides are in elements. */
+int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row_stride, uint64_t k_head_stride,
+                          const void* v, uint64_t v_row_stride, uint64_t v_head_stride, int dtype, void* k_cache,
+                          void* v_cache, int cache_dtype, uint64_t page_stride, uint64_t row_stride,
+                          uint64_t head_stride, uint32_t pages, uint32_t page_size, const int64_t* slot,
+                          uint32_t heads, uint32_t dim, uint32_t tokens, char* err, size_t errlen);
+
+/* Bytes of workspace that the two attention calls below need for this head size (16-byte aligned, device memory; it
+ * need not be initialised and holds nothing between calls; calls whose kernels may overlap need one each).
+ * No counterpart in the reference. */
+uint64_t halo_b200_attention_workspace(uint32_t dim);
+
+/* No counterpart in the reference's kernel boundary (its engine attends in src/model/qwen35.cpp:256-286): attention over packed
+ * prompts. Sequence b owns rows cu[b] .. cu[b + 1] of q [tokens][q_heads][dim], k, v [tokens][kv_heads][dim] and
+ * out [tokens][q_heads][dim]; query head h reads K/V head h / (q_heads / kv_heads);
+ *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * <q, k_j>),
+ * over the sequence's rows j, up to the query's own when causal is 1. lse (optional, [tokens][q_heads]) =
+ * log sum_j p_j. A query that sees no key gets zeros and -inf. Rows behind cu[batch] are neither read nor written.
+ * cu rises from 0 and stays within tokens (what lies beyond is cut).
+ * dtype f16 or bf16 for q, k, v and out; dim a multiple of 8 up to 256; q_heads / kv_heads a whole number up to 128;
+ * scale > 0. Strides in elements, multiples of 8; pointers 16-byte aligned. Products are exact in fp32 sums; p is
+ * rounded to dtype for the second product, out once from fp32. Values behind a mask never reach the result as long as
+ * they are finite; a V row that is not finite reaches the queries of a tile in which some query sees it. The same call
+ * gives the same bits. */
+int halo_b200_attention_packed(halo_b200_stream stream, const void* q, uint64_t q_row_stride, uint64_t q_head_stride,
+                               const void* k, uint64_t k_row_stride, uint64_t k_head_stride, const void* v,
+                               uint64_t v_row_stride, uint64_t v_head_stride, void* out, uint64_t out_row_stride,
+                               uint64_t out_head_stride, int dtype, const uint32_t* cu, uint32_t batch,
+                               uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t dim, float scale,
+                               int causal, float* lse, void* workspace, uint64_t workspace_bytes, char* err,
+                               size_t errlen);
+
+/* No counterpart in the reference's kernel boundary (src/model/qwen35.cpp:256-286): the same for new tokens over a paged cache,
+ * whose rows the new tokens' K and V already are (halo_b200_paged_store). Sequence b has the kv_len[b] newest keys in
+ * the pages table[b * table_stride + j / page_size], row j % page_size; with n = cu[b + 1] - cu[b] query rows, row i
+ * sees keys j <= kv_len[b] - n + i when causal is 1 (a single token all of them), else all. kv_len is cut at
+ * table_cols * page_size. Table entries behind the last key are not read, cache rows behind it do not count, whatever
+ * they hold. An entry outside 0 .. pages - 1 reads as zeros. Cache strides as in halo_b200_paged_store, multiples of 8. */
+int halo_b200_attention_paged(halo_b200_stream stream, const void* q, uint64_t q_row_stride, uint64_t q_head_stride,
+                              const void* k_cache, const void* v_cache, uint64_t page_stride, uint64_t row_stride,
+                              uint64_t head_stride, uint32_t pages, uint32_t page_size, const int32_t* table,
+                              uint64_t table_stride, uint32_t table_cols, const uint32_t* kv_len, void* out,
+                              uint64_t out_row_stride, uint64_t out_head_stride, int dtype, const uint32_t* cu,
+                              uint32_t batch, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t dim,
+                              float scale, int causal, float* lse, void* workspace, uint64_t workspace_bytes,
+                              char* err, size_t errlen);
+
 /* ---- launch by kernel name -------------------------------------------------------------- */
 
 /* One launch argument, as rt::Arg (src/rt/device.hpp:35-59): a device pointer (buffer base +
