@@ -47,24 +47,31 @@ constexpr uint32_t kMaxCtas = 148;
 constexpr float kLazy = 8.0f;      // log2 of the growth that a reference may lag behind
 constexpr uint32_t kTmemO = 256;   // TMEM columns: S0 0.., S1 128.., O 256..
 
-template <int D>
+// CG CTAs (a pair of neighbouring SMs, or one) work on a tile of CG x 128 rows. A pair's tensor cores share the
+// operands: each CTA stages half of K (its keys) and half of V (its columns), which halves both the traffic from L2 and
+// the reads of shared memory that bound a single CTA at these tile sizes.
+template <int D, int CG>
 struct Shape {
-  static constexpr uint32_t kKeys = D == 256 ? 64 : 128;        // keys of a tile
-  static constexpr uint32_t kStageBytes = kKeys * D * 2;        // 32, 32, 16 KB
+  static constexpr uint32_t kKeys = D == 256 && CG == 1 ? 64 : 128;    // keys of a tile
+  static constexpr uint32_t kStageBytes = kKeys * D * 2 / CG;          // one CTA's share of a tile of K or V
   static constexpr uint32_t kQBytes = kRows * D * 2;
-  static constexpr uint32_t kStages = D == 256 ? 5 : D == 128 ? 6 : 8;
+  static constexpr uint32_t kStages = kStageBytes == 32768 ? 5 : 8;
+  static constexpr uint32_t kKeyRows = kKeys / CG, kVChunks = D / 64 / CG;
+  static constexpr uint32_t kParts = kKeys / 64;                       // P is handed on in parts of 64 keys
 };
 
 struct alignas(16) Shared {
-  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_empty, m_full[2][4];
+  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty, m_full[2][4];
   uint32_t tmem, abort;
   uint32_t start[4], end[4];  // (sequence, K/V head, row tile, key tile) of the piece's borders
   float m[2][kRows];
   float l[2][kRows];
 };
-template <int D>
-constexpr uint32_t kSmemBytes = Shape<D>::kQBytes + Shape<D>::kStages * Shape<D>::kStageBytes + static_cast<uint32_t>(sizeof(Shared));
-static_assert(kSmemBytes<256> <= 232448 && kSmemBytes<128> <= 232448 && kSmemBytes<64> <= 232448, "shared memory of an SM");
+template <int D, int CG>
+constexpr uint32_t kSmemBytes = Shape<D, CG>::kQBytes + Shape<D, CG>::kStages * Shape<D, CG>::kStageBytes + static_cast<uint32_t>(sizeof(Shared));
+static_assert(kSmemBytes<256, 1> <= 232448 && kSmemBytes<256, 2> <= 232448 && kSmemBytes<128, 1> <= 232448 && kSmemBytes<128, 2> <= 232448 &&
+                  kSmemBytes<64, 1> <= 232448,
+              "shared memory of an SM");
 
 // ---- PTX ----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bar_init(unsigned long long* b, uint32_t n) {
@@ -87,20 +94,57 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// The same barrier in the CTA of rank 0 of the cluster.
+__device__ __forceinline__ void bar_arrive_leader(unsigned long long* b) {
+  asm volatile(
+      "{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, 0;\n"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(smem_addr(b))
+      : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// All threads of the CTA, or of both CTAs of a pair.
+template <int CG>
+__device__ __forceinline__ void sync_all() {
+  if constexpr (CG == 2) cluster_sync();
+  else __syncthreads();
+}
+// An arrival on `bar` (in both CTAs of a pair) once the products issued so far are done.
+template <int CG>
 __device__ __forceinline__ void tc_commit(unsigned long long* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+template <int CG>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
 }
+template <int CG>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
 }
 // 32 columns of this warp's 32 TMEM lanes. The results are only valid after tc_wait_ld().
 __device__ __forceinline__ void tc_ld32(uint32_t addr, float (&v)[32]) {
@@ -157,7 +201,7 @@ __device__ __forceinline__ void wait(Shared& sh, unsigned long long* b, uint32_t
   uint32_t done = 0;
   for (uint32_t spin = 0; spin < kStageSpinLimit && !done; ++spin) {
     asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
@@ -360,26 +404,29 @@ __device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <typename T, int D>
+template <typename T, int D, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using Sh = Shape<D>;
+  using Sh = Shape<D, CG>;
   constexpr uint32_t KT = Sh::kKeys, ST = Sh::kStages, kChunks = D / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw + Sh::kQBytes + ST * Sh::kStageBytes);
   const uint32_t q_smem = smem_addr(smem_raw), kv_smem = q_smem + Sh::kQBytes;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t tq = kRows / c.group;  // tokens of a row tile
+  const uint32_t rank = CG == 2 ? blockIdx.x & 1u : 0u, unit = blockIdx.x / CG, units = gridDim.x / CG;
+  const uint32_t tq_cta = kRows / c.group, tq = CG * tq_cta;  // tokens of a CTA's rows, of a row tile
 
   if (threadIdx.x == 0) {
-    for (uint32_t i = 0; i < ST; ++i) bar_init(&sh.kv_full[i], 1), bar_init(&sh.kv_empty[i], 1);
-    bar_init(&sh.q_full, 1);
+    // a pair's products need both CTAs' operands: the leader's barriers count the other's arrivals too
+    const uint32_t both = rank == 0 ? CG : 1;
+    for (uint32_t i = 0; i < ST; ++i) bar_init(&sh.kv_full[i], both), bar_init(&sh.kv_empty[i], 1);
+    bar_init(&sh.q_full, both);
     bar_init(&sh.q_empty, 1);
-    bar_init(&sh.o_empty, 8);
+    bar_init(&sh.o_empty, 8 * CG);
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.s_full[i], 1);
-      bar_init(&sh.p_full[i], 4);
+      for (int w = 0; w < 2; ++w) bar_init(&sh.p_full[i][w], 4 * CG);
       bar_init(&sh.pv_done[i], 1);
       for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1);
     }
@@ -387,12 +434,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   pdl_wait_and_trigger();
   if (warp < 2) {
-    // all of the work, and this CTA's borders (warp 0 the first, warp 1 the last)
+    // all of the work, and this unit's borders (warp 0 the first, warp 1 the last)
     unsigned long long w = 0;
     for (uint32_t b = lane; b < c.batch; b += 32) {
       const Seq s = load_seq(c, b, tq);
@@ -401,34 +453,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
     const unsigned long long most = (w + kMinShare - 1) / kMinShare;
-    const uint32_t n = static_cast<uint32_t>(min(static_cast<unsigned long long>(gridDim.x), most ? most : 1ull));
-    const uint32_t x = blockIdx.x + warp;
+    const uint32_t n = static_cast<uint32_t>(min(static_cast<unsigned long long>(units), most ? most : 1ull));
+    const uint32_t x = unit + warp;
     uint32_t at[4] = {c.batch, 0, 0, 0};
     if (x < n) locate<KT>(c, w / n * x + w % n * x / n, tq, at);
     if (lane < 4) (warp ? sh.end : sh.start)[lane] = lane == 0 ? at[0] : lane == 1 ? at[1] : lane == 2 ? at[2] : at[3];
   }
   tc_before();
-  __syncthreads();
+  sync_all<CG>();
   tc_after();
   const uint32_t tmem = sh.tmem;
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  Pieces<KT> pc(c, sh, tq);
-  if (warp == 8) {
-    // ---- copies -------------------------------------------------------------------------------------------------
-    if (lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    Pieces<KT> pc(c, sh, tq);
+    if (warp == 8 && lane == 0) {
+      // ---- copies -------------------------------------------------------------------------------------------------
       uint32_t g = 0, fill = 0, job = 0;
-      uint32_t issued = 0;  // loads whose completion nobody may wait for after an abort
-      const uint32_t q_bytes = kRows / c.group * c.group * 128u * kChunks;
-      auto load_kv = [&](const CUtensorMap* map, const Seq& s, uint32_t b, uint32_t h, uint32_t t, uint32_t keys, uint32_t seq) {
+      uint32_t issued = 0;  // stages that have had a load
+      const uint32_t q_bytes = tq_cta * c.group * 128u * kChunks;
+      // One operand's tile: `rows` key rows from `key0` on, chunks of 64 columns from `col` on, laid out [chunk][row].
+      auto load_kv = [&](const CUtensorMap* map, const Seq& s, uint32_t b, uint32_t h, uint32_t key0, uint32_t most, uint32_t keys, uint32_t col,
+                         uint32_t chunks, uint32_t seq) {
         const uint32_t st = seq % ST;
         if (seq >= ST) wait(sh, &sh.kv_empty[st], (seq / ST - 1) & 1u);
         if (aborted(sh)) return;
-        const uint32_t base = kv_smem + st * Sh::kStageBytes, key0 = t * KT;
+        const uint32_t base = kv_smem + st * Sh::kStageBytes;
         // rows behind the last visible key are left out by whole boxes
-        const uint32_t rows = min(KT, keys - key0), boxes = (rows + c.box_rows - 1) / c.box_rows;
-        stage_expect(smem_addr(&sh.kv_full[st]), boxes * c.box_rows * 128u * kChunks);
+        const uint32_t rows = keys > key0 ? min(most, keys - key0) : 0u, boxes = (rows + c.box_rows - 1) / c.box_rows;
+        stage_expect(smem_addr(&sh.kv_full[st]), boxes * c.box_rows * 128u * chunks);
         issued |= 1u << st;
         for (uint32_t x = 0; x < boxes; ++x) {
           const uint32_t key = key0 + x * c.box_rows;
@@ -437,8 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             page = c.table[b * c.table_stride + (key >> c.page_shift)];
             row = static_cast<int>(key & ((1u << c.page_shift) - 1u));
           }
-          for (uint32_t ch = 0; ch < kChunks; ++ch)
-            tma_4d(base + ch * KT * 128u + x * c.box_rows * 128u, map, static_cast<int>(ch * 64), row, static_cast<int>(h), page, &sh.kv_full[st]);
+          for (uint32_t ch = 0; ch < chunks; ++ch)
+            tma_4d(base + (ch * most + x * c.box_rows) * 128u, map, static_cast<int>(col + ch * 64), row, static_cast<int>(h), page, &sh.kv_full[st]);
         }
       };
       // order of use: K(0), K(1), V(0), K(2), V(1), ...
@@ -447,21 +500,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; pc.next() && !aborted(sh); pc.advance()) {
         for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
           const uint32_t kslot = fill++;
-          if (g > 0) load_kv(&vmap, ps, pb, ph, pt, pkeys, fill++);
+          if (g > 0) load_kv(&vmap, ps, pb, ph, pt * KT, KT, pkeys, rank * (D / CG), Sh::kVChunks, fill++);
           if (t == pc.t0) {
             if (job > 0) wait(sh, &sh.q_empty, (job - 1) & 1u);
             if (aborted(sh)) break;
             stage_expect(smem_addr(&sh.q_full), q_bytes);
             for (uint32_t ch = 0; ch < kChunks; ++ch)
               tma_3d(q_smem + ch * kRows * 128u, &qmap, static_cast<int>(ch * 64), static_cast<int>(pc.h * c.group),
-                     static_cast<int>(pc.s.row0 + pc.i * tq), &sh.q_full);
+                     static_cast<int>(pc.s.row0 + pc.i * tq + rank * tq_cta), &sh.q_full);
             ++job;
           }
-          load_kv(&kmap, pc.s, pc.b, pc.h, t, pc.keys, kslot);
+          load_kv(&kmap, pc.s, pc.b, pc.h, t * KT + rank * Sh::kKeyRows, Sh::kKeyRows, pc.keys, 0, kChunks, kslot);
           ps = pc.s, pb = pc.b, ph = pc.h, pt = t, pkeys = pc.keys;
         }
       }
-      if (g > 0 && !aborted(sh)) load_kv(&vmap, ps, pb, ph, pt, pkeys, fill++);
+      if (g > 0 && !aborted(sh)) load_kv(&vmap, ps, pb, ph, pt * KT, KT, pkeys, rank * (D / CG), Sh::kVChunks, fill++);
+      // every stage's last use is over before the CTA may leave: no arrival of the other CTA's products is under way
+      if (!aborted(sh)) {
+        for (uint32_t i = fill > ST ? fill - ST : 0u; i < fill; ++i) wait(sh, &sh.kv_empty[i % ST], (i / ST) & 1u);
+        if (job) wait(sh, &sh.q_empty, (job - 1) & 1u);
+      }
       if (aborted(sh)) {
         // no copy may land in shared memory that another CTA owns by then: one more bounded wait for each
         for (uint32_t st = 0; st < ST; ++st)
@@ -474,78 +532,98 @@ __global__ void __launch_bounds__(kThreads, 1)
           stage_wait(smem_addr(&sh.q_full), 1);
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    // ---- matrix products ----------------------------------------------------------------------------------------
-    constexpr uint32_t idesc_s = instr_desc<T>(kRows, KT, false), idesc_o = instr_desc<T>(kRows, D, true);
-    uint32_t g = 0, fill = 0, job = 0;
-    uint32_t prev_first = 0, prev_valid = 0, prev_job = 0;  // of tile g - 1
-    auto pv = [&](uint32_t gt, uint32_t slot, bool first, uint32_t valid, uint32_t jobno) {
-      const uint32_t st = slot % ST, buf = gt & 1u, base = kv_smem + st * Sh::kStageBytes;
-      wait(sh, &sh.kv_full[st], (slot / ST) & 1u);
-      if (valid < KT) {
-        // V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: clear them
-        for (uint32_t x = lane; x < (KT - valid) * 8u * kChunks; x += 32) {
-          const uint32_t ch = x / ((KT - valid) * 8u), y = x - ch * ((KT - valid) * 8u);
-          const uint32_t at = base + ch * KT * 128u + valid * 128u + y * 16u;
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+    } else if (warp == 9) {
+      // ---- matrix products (the pair's leader), or word to the leader that this CTA's operands are there ----------
+      constexpr uint32_t idesc_s = instr_desc<T>(CG * kRows, KT, false), idesc_o = instr_desc<T>(CG * kRows, D, true);
+      const bool leader = rank == 0;
+      uint32_t g = 0, fill = 0, job = 0;
+      uint32_t prev_first = 0, prev_valid = 0, prev_job = 0;  // of tile g - 1
+      auto pv = [&](uint32_t gt, uint32_t slot, bool first, uint32_t valid, uint32_t jobno) {
+        const uint32_t st = slot % ST, buf = gt & 1u, base = kv_smem + st * Sh::kStageBytes;
+        wait(sh, &sh.kv_full[st], (slot / ST) & 1u);
+        if (valid < KT) {
+          // V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: clear them
+          const uint32_t per = (KT - valid) * 8u;
+          for (uint32_t x = lane; x < per * Sh::kVChunks; x += 32) {
+            const uint32_t ch = x / per, at = base + (ch * KT + valid) * 128u + (x - ch * per) * 16u;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
-      if (first && jobno > 0) wait(sh, &sh.o_empty, (jobno - 1) & 1u);
-      wait(sh, &sh.p_full[buf], (gt >> 1) & 1u);
-      tc_after();
-      if (lane == 0 && !aborted(sh)) {
+        if (!leader) {
+          if (lane == 0) bar_arrive_leader(&sh.kv_full[st]);
+          return;
+        }
+        if (first && jobno > 0) wait(sh, &sh.o_empty, (jobno - 1) & 1u);
         const uint64_t vd = smem_desc(base, KT * 128u);
 #pragma unroll
-        for (uint32_t k = 0; k < KT / 16; ++k)
-          mma_ts(tmem + kTmemO, tmem + buf * 128u + k * 8u, vd + k * (2048u >> 4), idesc_o, !(first && k == 0));
-        tc_commit(&sh.kv_empty[st]);
-        tc_commit(&sh.pv_done[buf]);
-      }
-      __syncwarp();
-    };
-    uint32_t vslot = 0;
-    for (; pc.next() && !aborted(sh); pc.advance()) {
-      for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
-        const uint32_t kslot = fill++, buf = g & 1u, st = kslot % ST;
-        if (g > 0) vslot = fill++;
-        if (t == pc.t0) wait(sh, &sh.q_full, job & 1u);
-        wait(sh, &sh.kv_full[st], (kslot / ST) & 1u);
-        tc_after();
-        if (lane == 0 && !aborted(sh)) {
-          const uint64_t qd = smem_desc(q_smem, 16), kd = smem_desc(kv_smem + st * Sh::kStageBytes, 16);
+        for (uint32_t part = 0; part < Sh::kParts; ++part) {
+          wait(sh, &sh.p_full[buf][part], (gt >> 1) & 1u);
+          tc_after();
+          if (lane == 0 && !aborted(sh)) {
 #pragma unroll
-          for (uint32_t k = 0; k < D / 16; ++k)
-            mma_ss(tmem + buf * 128u, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u, kd + ((k >> 2) * KT * 128u + (k & 3u) * 32u) / 16u,
-                   idesc_s, k > 0);
-          tc_commit(&sh.kv_empty[st]);
-          tc_commit(&sh.s_full[buf]);
-          if (t + 1 == pc.t1) tc_commit(&sh.q_empty);
+            for (uint32_t k = part * 4; k < part * 4 + 4; ++k)
+              mma_ts<CG>(tmem + kTmemO, tmem + buf * 128u + k * 8u, vd + k * (2048u >> 4), idesc_o, !(first && k == 0));
+            if (part + 1 == Sh::kParts) {
+              tc_commit<CG>(&sh.kv_empty[st]);
+              tc_commit<CG>(&sh.pv_done[buf]);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (g > 0) pv(g - 1, vslot, prev_first != 0, prev_valid, prev_job);
-        prev_first = t == pc.t0;
-        prev_valid = min(KT, pc.keys - t * KT);
-        prev_job = job;
+      };
+      uint32_t vslot = 0;
+      for (; pc.next() && !aborted(sh); pc.advance()) {
+        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
+          const uint32_t kslot = fill++, buf = g & 1u, st = kslot % ST;
+          if (g > 0) vslot = fill++;
+          if (t == pc.t0) wait(sh, &sh.q_full, job & 1u);
+          wait(sh, &sh.kv_full[st], (kslot / ST) & 1u);
+          if (!leader) {
+            if (lane == 0) {
+              if (t == pc.t0) bar_arrive_leader(&sh.q_full);
+              bar_arrive_leader(&sh.kv_full[st]);
+            }
+          } else {
+            tc_after();
+            if (lane == 0 && !aborted(sh)) {
+              const uint64_t qd = smem_desc(q_smem, 16), kd = smem_desc(kv_smem + st * Sh::kStageBytes, 16);
+#pragma unroll
+              for (uint32_t k = 0; k < D / 16; ++k)
+                mma_ss<CG>(tmem + buf * 128u, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u,
+                           kd + ((k >> 2) * Sh::kKeyRows * 128u + (k & 3u) * 32u) / 16u, idesc_s, k > 0);
+              tc_commit<CG>(&sh.kv_empty[st]);
+              tc_commit<CG>(&sh.s_full[buf]);
+              if (t + 1 == pc.t1) tc_commit<CG>(&sh.q_empty);
+            }
+          }
+          __syncwarp();
+          if (g > 0) pv(g - 1, vslot, prev_first != 0, prev_valid, prev_job);
+          prev_first = t == pc.t0;
+          prev_valid = min(KT, pc.keys - t * KT);
+          prev_job = job;
+        }
+        if (pc.t1 > pc.t0) ++job;
       }
-      if (pc.t1 > pc.t0) ++job;
+      if (g > 0 && !aborted(sh)) pv(g - 1, fill++, prev_first != 0, prev_valid, prev_job);
     }
-    if (g > 0 && !aborted(sh)) pv(g - 1, fill++, prev_first != 0, prev_valid, prev_job);
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     Pieces<KT> pc(c, sh, tq);
+    auto tell_leader = [&](unsigned long long* b) {
+      if (rank == 0) bar_arrive(b);
+      else bar_arrive_leader(b);
+    };
     // ---- softmax, and the outputs -------------------------------------------------------------------------------
     const uint32_t wg = warp >> 2, quad = warp & 3u, row = quad * 32u + lane;
     const uint32_t lane_base = (quad * 32u) << 16;
     const uint32_t my_tok = row / c.group, my_head = row - my_tok * c.group;
     uint32_t g = 0;
-    if (threadIdx.x == 0) c.meta[8u * blockIdx.x] = c.meta[8u * blockIdx.x + 1] = 0;
+    if (threadIdx.x == 0 && rank == 0) c.meta[8u * unit] = c.meta[8u * unit + 1] = 0;
     for (; pc.next(); pc.advance()) {
-      const uint32_t tok0 = pc.i * tq, toks = min(tq, pc.s.rows - tok0), rows = toks * c.group;
+      const uint32_t tok0 = pc.i * tq + rank * tq_cta;
+      const uint32_t rows = tok0 < pc.s.rows ? min(tq_cta, pc.s.rows - tok0) * c.group : 0u;  // of this CTA
       const bool busy = quad * 32u < rows;  // warps without a row only keep step
       // keys that this row sees
       uint32_t limit = pc.keys;
@@ -618,6 +696,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               r[y] = pack2<T>(v.x, v.y);
             }
             tc_st32(tmem + lane_base + buf * 128u + x * 32u, r);
+            if (x + 1 < Sh::kParts) {  // the first part goes to the tensor cores while the second is computed
+              tc_wait_st();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) tell_leader(&sh.p_full[buf][x]);
+            }
           }
           if (next_ref != m) {
             if (m != -INFINITY) l = __fmul_rn(l, ex2_approx(__fmul_rn(m - next_ref, c.scale_log2)));
@@ -626,11 +710,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           l += sum.x + sum.y;
           tc_wait_st();
         } else {
-          if (lane == 0) bar_arrive(&sh.m_full[buf][quad]);
+          if (lane == 0) {
+            bar_arrive(&sh.m_full[buf][quad]);
+            for (uint32_t x = 0; x + 1 < Sh::kParts; ++x) tell_leader(&sh.p_full[buf][x]);
+          }
         }
         tc_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&sh.p_full[buf]);
+        if (lane == 0) tell_leader(&sh.p_full[buf][Sh::kParts - 1]);
       }
       // the two groups' denominators over one reference, the last tile's
       const bool any = pc.t1 > pc.t0;
@@ -655,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kHalf = D / 2;  // columns of a group
       if (busy) {
         float* piece = nullptr;
-        if (!whole) piece = c.part + (2ull * blockIdx.x + (pc.t0 == 0 ? 1u : 0u)) * AttnPieceFloats(D);
+        if (!whole) piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
 #pragma unroll 1
         for (uint32_t x = 0; x < kHalf / 32; ++x) {
           const uint32_t col = wg * kHalf + x * 32u;
@@ -703,21 +790,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_before();
       __syncwarp();
-      if (any && lane == 0) bar_arrive(&sh.o_empty);
+      if (any && lane == 0) tell_leader(&sh.o_empty);
       asm volatile("bar.sync 1, 256;" ::: "memory");  // before sh.l is written again
-      if (threadIdx.x == 0 && !whole) {
+      if (threadIdx.x == 0 && rank == 0 && !whole) {
         // what the join needs: a piece that opens a split job says which one, every other one whether it ends it
-        uint32_t* to = c.meta + 8u * blockIdx.x;
+        uint32_t* to = c.meta + 8u * unit;
         if (pc.t0 == 0) to[1] = 1u, to[2] = pc.b, to[3] = pc.h, to[4] = pc.i;
         else to[0] = pc.t1 == pc.n ? 2u : 1u;
       }
     }
   }
 
+  __syncwarp();
   tc_before();
-  __syncthreads();
+  sync_all<CG>();
   tc_after();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == 9) {
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
 }
 
 
@@ -727,8 +818,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // pieces (a prompt's jobs are cut once): a warp sums a column quad over all of them; many (one token over a long cache
 // is cut by every CTA): the warps share the pieces and meet in shared memory. The order of the sums is fixed.
 constexpr uint32_t kJoinWarps = 8;
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnCall c, const uint32_t ctas) {
+template <typename T, int D, int CG>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnCall c, const uint32_t units) {
   __shared__ uint32_t opens[(kMaxCtas + 31) / 32], ends[(kMaxCtas + 31) / 32];
   __shared__ float weight[kMaxCtas + 1][32];
   __shared__ float4 red[kJoinWarps][32];
@@ -736,7 +827,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
   pdl_wait_and_trigger();
   if (warp < (kMaxCtas + 31) / 32) {
     const uint32_t x = warp * 32u + lane;
-    const uint32_t f0 = x < ctas ? c.meta[8u * x] : 0u, f1 = x < ctas ? c.meta[8u * x + 1] : 0u;
+    const uint32_t f0 = x < units ? c.meta[8u * x] : 0u, f1 = x < units ? c.meta[8u * x + 1] : 0u;
     const uint32_t o = __ballot_sync(kFullMask, f1 == 1u), e = __ballot_sync(kFullMask, f0 == 2u);
     if (lane == 0) opens[warp] = o, ends[warp] = e;
   }
@@ -752,7 +843,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
     }
     k -= n;
   }
-  if (first >= ctas) return;
+  if (first >= units) return;
   uint32_t last = first;
   for (uint32_t w = (first + 1) / 32; w < (kMaxCtas + 31) / 32; ++w) {
     uint32_t v = ends[w];
@@ -764,13 +855,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
   }
   const uint32_t pieces = last - first + 1;
   const uint32_t* job = c.meta + 8u * first;
-  const uint32_t h = job[3], tq = kRows / c.group, tok0 = job[4] * tq;
-  const Seq s = load_seq(c, job[2], tq);
-  const uint32_t rows = min(tq, s.rows - tok0) * c.group;
-  const uint32_t row = (blockIdx.y & 3u) * 32u + lane;
-  if ((blockIdx.y & 3u) * 32u >= rows) return;
+  const uint32_t tq_cta = kRows / c.group, group = blockIdx.y % (4 * CG), rank = group >> 2;
+  const uint32_t h = job[3], tok0 = job[4] * CG * tq_cta + rank * tq_cta;
+  const Seq s = load_seq(c, job[2], CG * tq_cta);
+  const uint32_t rows = tok0 < s.rows ? min(tq_cta, s.rows - tok0) * c.group : 0u;
+  const uint32_t row = (group & 3u) * 32u + lane;
+  if ((group & 3u) * 32u >= rows) return;
   // piece 0 opened the job, the others are what the CTAs behind began with
-  auto piece = [&](uint32_t p) { return c.part + (2ull * (first + p) + (p == 0 ? 1u : 0u)) * AttnPieceFloats(D); };
+  auto piece = [&](uint32_t p) { return c.part + ((2ull * (first + p) + (p == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D); };
   for (uint32_t p = warp; p < pieces; p += kJoinWarps) weight[p][lane] = row < rows ? piece(p)[D * kRows + row] : -INFINITY;
   __syncthreads();
   float top = -INFINITY;
@@ -797,12 +889,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
   const uint64_t token = s.row0 + tok0 + row / c.group;
   const uint32_t head = h * c.group + row % c.group;
   T* out = static_cast<T*>(c.out) + token * c.out_row + head * c.out_head;
-  if (c.lse && blockIdx.y < 4 && warp == 0 && row < rows)
+  if (c.lse && blockIdx.y < 4 * CG && warp == 0 && row < rows)
     c.lse[token * (c.kv_heads * c.group) + head] =
         total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total)), 0.69314718055994531f);
   const bool shared = pieces > 4;
   const uint32_t p0 = shared ? warp : 0u, pstep = shared ? kJoinWarps : 1u;
-  const uint32_t parts = gridDim.y >> 2, quads = D / 4 / parts, q0 = (blockIdx.y >> 2) * quads;
+  const uint32_t parts = gridDim.y / (4 * CG), quads = D / 4 / parts, q0 = blockIdx.y / (4 * CG) * quads;
   for (uint32_t q = q0 + (shared ? 0u : warp); q < q0 + quads; q += shared ? 1u : kJoinWarps) {
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (row < rows) {
@@ -870,7 +962,7 @@ constexpr uint64_t kMetaBytes = 8192;
 static_assert(kMetaBytes >= kMaxCtas * 32, "eight words for each CTA");
 constexpr uint32_t PadDim(uint32_t dim) { return dim <= 64 ? 64u : dim <= 128 ? 128u : 256u; }
 
-template <typename T, int D>
+template <typename T, int D, int CG>
 cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   AttnCall c{};
   c.cu = a.cu;
@@ -892,12 +984,12 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   c.lse = a.lse;
   c.meta = static_cast<uint32_t*>(a.workspace);
   c.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kMetaBytes);
-  const uint32_t tq = kRows / c.group;
+  const uint32_t tq_cta = kRows / c.group, tq = CG * tq_cta;
   c.box_rows = a.table && (1u << a.page_shift) < 64u ? 1u << a.page_shift : 64u;
 
   CUtensorMap qm, km, vm;
   const uint64_t qd[3] = {a.dim, a.q_heads, a.tokens}, qs[3] = {1, a.q_head, a.q_row};
-  const uint32_t qb[3] = {64, c.group, tq};
+  const uint32_t qb[3] = {64, c.group, tq_cta};
   cudaError_t e = MakeMap(&qm, a.dtype, a.q, 3, qd, qs, qb);
   if (e != cudaSuccess) return e;
   const uint64_t rows = a.table ? uint64_t{1} << a.page_shift : a.tokens, pages = a.table ? a.pages : 1;
@@ -912,30 +1004,51 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes<D>));
+    e = cudaFuncSetAttribute(attention_kernel<T, D, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes<D, CG>));
   if (e != cudaSuccess) return e;
   const uint64_t most_keys = a.table ? static_cast<uint64_t>(a.table_cols) << a.page_shift : a.tokens;
   const uint64_t jobs = (static_cast<uint64_t>(a.tokens) / tq + a.batch) * a.kv_heads;  // at most
-  const uint64_t tiles = (most_keys + Shape<D>::kKeys - 1) / Shape<D>::kKeys;
-  uint64_t ctas = (jobs * (tiles + kJobCost) + kMinShare - 1) / kMinShare;
-  if (ctas > static_cast<uint64_t>(sms)) ctas = static_cast<uint64_t>(sms);
-  if (ctas > kMaxCtas) ctas = kMaxCtas;
-  if (ctas < 1) ctas = 1;
-  e = LaunchKernel(attention_kernel<T, D>, static_cast<unsigned>(ctas), kThreads, kSmemBytes<D>, s, c, qm, km, vm);
+  const uint64_t tiles = (most_keys + Shape<D, CG>::kKeys - 1) / Shape<D, CG>::kKeys;
+  uint64_t units = (jobs * (tiles + kJobCost) + kMinShare - 1) / kMinShare;
+  const uint64_t most_units = static_cast<uint64_t>(sms < static_cast<int>(kMaxCtas) ? sms : static_cast<int>(kMaxCtas)) / CG;
+  if (units > most_units) units = most_units;
+  if (units < 1) units = 1;
+
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = static_cast<unsigned>(units * CG);
+  cfg.blockDim = kThreads;
+  cfg.dynamicSmemBytes = kSmemBytes<D, CG>;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PdlEnabled() ? 2u : 1u;
+  e = cudaLaunchKernelEx(&cfg, attention_kernel<T, D, CG>, c, qm, km, vm);
   // jobs of one tile are never split
-  if (e != cudaSuccess || tiles <= 1 || ctas == 1) return e;
-  const uint32_t x = static_cast<uint32_t>(jobs < ctas ? jobs : ctas);
+  if (e != cudaSuccess || tiles <= 1 || units == 1) return e;
+  const uint32_t x = static_cast<uint32_t>(jobs < units ? jobs : units);
   uint32_t parts = 1;
-  while (parts < 16 && x * 4 * parts * 2 <= 148 * 8) parts *= 2;
-  return LaunchKernel(attention_join_kernel<T, D>, dim3(x, 4 * parts), kJoinWarps * 32, 0, s, c, static_cast<uint32_t>(ctas));
+  while (parts < D / 16 && x * 4 * CG * parts * 2 <= 148 * 8) parts *= 2;
+  return LaunchKernel(attention_join_kernel<T, D, CG>, dim3(x, 4 * CG * parts), kJoinWarps * 32, 0, s, c, static_cast<uint32_t>(units));
+}
+
+// A pair's tile has twice the rows: it pays where a sequence's rows (tokens x heads of a group) fill more than one CTA's.
+template <typename T, int D>
+cudaError_t LaunchPair(const AttnArgs& a, cudaStream_t s) {
+  if (static_cast<uint64_t>(a.tokens) * (a.q_heads / a.kv_heads) > static_cast<uint64_t>(a.batch) * kRows) return Launch<T, D, 2>(a, s);
+  return Launch<T, D, 1>(a, s);
 }
 
 template <typename T>
 cudaError_t LaunchDim(const AttnArgs& a, cudaStream_t s) {
   switch (PadDim(a.dim)) {
-    case 64: return Launch<T, 64>(a, s);
-    case 128: return Launch<T, 128>(a, s);
-    default: return Launch<T, 256>(a, s);
+    case 64: return Launch<T, 64, 1>(a, s);
+    case 128: return LaunchPair<T, 128>(a, s);
+    default: return LaunchPair<T, 256>(a, s);
   }
 }
 
