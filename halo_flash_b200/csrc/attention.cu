@@ -18,7 +18,7 @@
 // needed; every CTA finds its piece from cu / kv_len by itself.
 //
 // Roles in a CTA (384 threads): warp 8 copies Q, K and V by TMA into shared memory (K and V through a ring of
-// stages), warp 9 issues the tcgen05.mma, warps 0-3 and 4-7 are two softmax groups that take alternate key tiles
+// stages), one thread of warp 9 issues the tcgen05.mma, warp 10 clears what no row may see of V, warps 0-3 and 4-7 are two softmax groups that take alternate key tiles
 // (thread = row), so that one group's exponentials run beside the other's TMEM traffic and the tensor cores.
 //
 // Waits are bounded as in stage.cuh: one that runs out sets a flag that makes the other waits return at once, the CTA
@@ -61,7 +61,7 @@ struct Shape {
 };
 
 struct alignas(16) Shared {
-  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty, m_full[2][4];
+  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty, v_dirty, v_clean, m_full[2][4];
   uint32_t tmem, abort;
   uint32_t start[4], end[4];  // (sequence, K/V head, row tile, key tile) of the piece's borders
   float m[2][kRows];
@@ -94,13 +94,23 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// The same barrier in the CTA of rank 0 of the cluster.
+// The same barrier in the CTA of rank 0 of the cluster. What it tells of lies in tensor memory, or came by TMA; cluster-scope
+// acquire and release on every wait and arrival cost about 300 cycles each (a tile of 128 keys took 4000 cycles instead of
+// 2500) and order nothing more than that needs. Where a thread's own stores are meant, fence.acq_rel.cluster stands before.
 __device__ __forceinline__ void bar_arrive_leader(unsigned long long* b) {
   asm volatile(
       "{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, 0;\n"
-      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(smem_addr(b))
+      "mbarrier.arrive.shared::cluster.b64 _, [r];\n}" ::"r"(smem_addr(b))
       : "memory");
 }
+// True in one thread of a converged warp. Operands of the tcgen05 instructions live in uniform registers: code that the
+// compiler can tell is warp-uniform, with this for a condition, keeps them there.
+__device__ __forceinline__ bool elect() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(kFullMask, v, 0); }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -201,7 +211,7 @@ __device__ __forceinline__ void wait(Shared& sh, unsigned long long* b, uint32_t
   uint32_t done = 0;
   for (uint32_t spin = 0; spin < kStageSpinLimit && !done; ++spin) {
     asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
@@ -413,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw + Sh::kQBytes + ST * Sh::kStageBytes);
   const uint32_t q_smem = smem_addr(smem_raw), kv_smem = q_smem + Sh::kQBytes;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const uint32_t rank = CG == 2 ? blockIdx.x & 1u : 0u, unit = blockIdx.x / CG, units = gridDim.x / CG;
   const uint32_t tq_cta = kRows / c.group, tq = CG * tq_cta;  // tokens of a CTA's rows, of a row tile
 
@@ -423,6 +433,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t i = 0; i < ST; ++i) bar_init(&sh.kv_full[i], both), bar_init(&sh.kv_empty[i], 1);
     bar_init(&sh.q_full, both);
     bar_init(&sh.q_empty, 1);
+    bar_init(&sh.v_dirty, 1);
+    bar_init(&sh.v_clean, 1);
     bar_init(&sh.o_empty, 8 * CG);
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.s_full[i], 1);
@@ -532,39 +544,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           stage_wait(smem_addr(&sh.q_full), 1);
         }
       }
-    } else if (warp == 9) {
-      // ---- matrix products (the pair's leader), or word to the leader that this CTA's operands are there ----------
+    } else if (warp == 9 && rank == 0) {
+      // ---- matrix products, issued by one thread (of the pair) -----------------------------------------------------
       constexpr uint32_t idesc_s = instr_desc<T>(CG * kRows, KT, false), idesc_o = instr_desc<T>(CG * kRows, D, true);
-      const bool leader = rank == 0;
-      uint32_t g = 0, fill = 0, job = 0;
-      uint32_t prev_first = 0, prev_valid = 0, prev_job = 0;  // of tile g - 1
-      auto pv = [&](uint32_t gt, uint32_t slot, bool first, uint32_t valid, uint32_t jobno) {
-        const uint32_t st = slot % ST, buf = gt & 1u, base = kv_smem + st * Sh::kStageBytes;
-        wait(sh, &sh.kv_full[st], (slot / ST) & 1u);
-        if (valid < KT) {
-          // V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: clear them
-          const uint32_t per = (KT - valid) * 8u;
-          for (uint32_t x = lane; x < per * Sh::kVChunks; x += 32) {
-            const uint32_t ch = x / per, at = base + (ch * KT + valid) * 128u + (x - ch * per) * 16u;
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
+      const uint32_t qs = uniform(q_smem), kvs = uniform(kv_smem), tm = uniform(tmem);
+      uint32_t g = 0, job = 0, tails = 0, st = 0, ph = 0;  // the stages are used in the order in which they are filled
+      uint32_t first = 0, tail = 0, prev_job = 0;          // of tile g - 1
+      auto next_stage = [&] {
+        if (++st == ST) st = 0, ph ^= 1u;
+      };
+      auto pv = [&](uint32_t gt) {
+        const uint32_t buf = uniform(gt & 1u);
+        const uint64_t d = smem_desc(kvs + uniform(st) * Sh::kStageBytes, KT * 128u);
+        const uint32_t acc = uniform(first) ^ 1u;
+        wait(sh, &sh.kv_full[st], ph);
+        if (tail) {
+          if (lane == 0) bar_arrive(&sh.v_dirty);
+          wait(sh, &sh.v_clean, tails++ & 1u);
         }
-        if (!leader) {
-          if (lane == 0) bar_arrive_leader(&sh.kv_full[st]);
-          return;
-        }
-        if (first && jobno > 0) wait(sh, &sh.o_empty, (jobno - 1) & 1u);
-        const uint64_t vd = smem_desc(base, KT * 128u);
+        if (first && prev_job > 0) wait(sh, &sh.o_empty, (prev_job - 1) & 1u);
 #pragma unroll
         for (uint32_t part = 0; part < Sh::kParts; ++part) {
           wait(sh, &sh.p_full[buf][part], (gt >> 1) & 1u);
           tc_after();
-          if (lane == 0 && !aborted(sh)) {
+          if (elect()) {
 #pragma unroll
             for (uint32_t k = part * 4; k < part * 4 + 4; ++k)
-              mma_ts<CG>(tmem + kTmemO, tmem + buf * 128u + k * 8u, vd + k * (2048u >> 4), idesc_o, !(first && k == 0));
+              mma_ts<CG>(tm + kTmemO, tm + buf * 128u + k * 8u, d + k * (2048u >> 4), idesc_o, k == 0 ? acc : 1u);
             if (part + 1 == Sh::kParts) {
               tc_commit<CG>(&sh.kv_empty[st]);
               tc_commit<CG>(&sh.pv_done[buf]);
@@ -572,41 +578,77 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         }
+        next_stage();
       };
-      uint32_t vslot = 0;
       for (; pc.next() && !aborted(sh); pc.advance()) {
-        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
-          const uint32_t kslot = fill++, buf = g & 1u, st = kslot % ST;
-          if (g > 0) vslot = fill++;
-          if (t == pc.t0) wait(sh, &sh.q_full, job & 1u);
-          wait(sh, &sh.kv_full[st], (kslot / ST) & 1u);
-          if (!leader) {
-            if (lane == 0) {
-              if (t == pc.t0) bar_arrive_leader(&sh.q_full);
-              bar_arrive_leader(&sh.kv_full[st]);
-            }
-          } else {
-            tc_after();
-            if (lane == 0 && !aborted(sh)) {
-              const uint64_t qd = smem_desc(q_smem, 16), kd = smem_desc(kv_smem + st * Sh::kStageBytes, 16);
+        const uint32_t t0 = uniform(pc.t0), t1 = uniform(pc.t1);
+        for (uint32_t t = t0; t < t1; ++t, ++g) {
+          const uint32_t buf = uniform(g & 1u);
+          const uint64_t qd = smem_desc(qs, 16), d = smem_desc(kvs + uniform(st) * Sh::kStageBytes, 16);
+          if (t == t0) wait(sh, &sh.q_full, job & 1u);
+          wait(sh, &sh.kv_full[st], ph);
+          if (elect()) {
 #pragma unroll
-              for (uint32_t k = 0; k < D / 16; ++k)
-                mma_ss<CG>(tmem + buf * 128u, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u,
-                           kd + ((k >> 2) * Sh::kKeyRows * 128u + (k & 3u) * 32u) / 16u, idesc_s, k > 0);
-              tc_commit<CG>(&sh.kv_empty[st]);
-              tc_commit<CG>(&sh.s_full[buf]);
-              if (t + 1 == pc.t1) tc_commit<CG>(&sh.q_empty);
-            }
+            for (uint32_t k = 0; k < D / 16; ++k)
+              mma_ss<CG>(tm + buf * 128u, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u,
+                         d + ((k >> 2) * Sh::kKeyRows * 128u + (k & 3u) * 32u) / 16u, idesc_s, k > 0);
+            tc_commit<CG>(&sh.kv_empty[st]);
+            tc_commit<CG>(&sh.s_full[buf]);
+            if (t + 1 == t1) tc_commit<CG>(&sh.q_empty);
           }
           __syncwarp();
-          if (g > 0) pv(g - 1, vslot, prev_first != 0, prev_valid, prev_job);
-          prev_first = t == pc.t0;
-          prev_valid = min(KT, pc.keys - t * KT);
+          next_stage();
+          if (g > 0) pv(g - 1);
+          first = t == t0;
+          tail = pc.keys - t * KT < KT;
           prev_job = job;
         }
-        if (pc.t1 > pc.t0) ++job;
+        if (t1 > t0) ++job;
       }
-      if (g > 0 && !aborted(sh)) pv(g - 1, fill++, prev_first != 0, prev_valid, prev_job);
+      if (g > 0 && !aborted(sh)) pv(g - 1);
+    } else if (warp == 10) {
+      // ---- V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: they are
+      // cleared. And a pair's second CTA tells the leader what has landed.
+      uint32_t g = 0, st = 0, ph = 0, jobs = 0, tails = 0, valid = KT;
+      auto next_stage = [&] {
+        if (++st == ST) st = 0, ph ^= 1u;
+      };
+      auto v_stage = [&] {
+        // the second CTA's stage waits for its word, the leader's only where the multiplying thread asked for it
+        if (rank) wait(sh, &sh.kv_full[st], ph);
+        else if (valid < KT) wait(sh, &sh.v_dirty, tails++ & 1u);
+        if (valid < KT) {
+          const uint32_t per = (KT - valid) * 8u, base = kv_smem + st * Sh::kStageBytes;
+          for (uint32_t x = lane; x < per * Sh::kVChunks; x += 32) {
+            const uint32_t ch = x / per, at = base + (ch * KT + valid) * 128u + (x - ch * per) * 16u;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (rank) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && rank == 0) bar_arrive(&sh.v_clean);
+        }
+        if (lane == 0 && rank) bar_arrive_leader(&sh.kv_full[st]);
+        __syncwarp();
+        next_stage();
+      };
+      for (; pc.next() && !aborted(sh); pc.advance()) {
+        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
+          if (rank) {
+            if (t == pc.t0) {
+              wait(sh, &sh.q_full, jobs++ & 1u);
+              if (lane == 0) bar_arrive_leader(&sh.q_full);
+            }
+            wait(sh, &sh.kv_full[st], ph);
+            if (lane == 0) bar_arrive_leader(&sh.kv_full[st]);
+            __syncwarp();
+          }
+          next_stage();
+          if (g > 0) v_stage();
+          valid = min(KT, pc.keys - t * KT);
+        }
+      }
+      if (g > 0 && !aborted(sh)) v_stage();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
