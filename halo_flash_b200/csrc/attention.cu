@@ -252,20 +252,21 @@ __device__ __forceinline__ uint32_t key_end(const AttnCall& c, const Seq& s, uin
   const int e = s.off + static_cast<int>(min(s.rows, (i + 1) * tq));
   return e > 0 ? static_cast<uint32_t>(e) : 0u;
 }
-// sum over i < n of floor((a i + b) / m), by Euclid's algorithm on (a, m).
-__device__ __forceinline__ unsigned long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  unsigned long long s = 0;
-  for (int guard = 0; guard < 64 && n; ++guard) {
-    if (a >= m) s += static_cast<unsigned long long>(n) * (n - 1) / 2 * (a / m), a %= m;
-    if (b >= m) s += static_cast<unsigned long long>(n) * (b / m), b %= m;
-    const unsigned long long y = static_cast<unsigned long long>(a) * n + b;
-    if (y < m) break;
-    n = static_cast<uint32_t>(y / m);
-    b = static_cast<uint32_t>(y % m);
-    const uint32_t t = m;
+// sum over i < n of floor((a i + b) / M) for a power of two M, by Euclid's algorithm on (a, M). a n + b < 2^32.
+template <uint32_t M>
+__device__ __forceinline__ unsigned long long floor_sum(uint32_t n, uint32_t a, uint32_t b) {
+  auto pairs = [](uint32_t k) { return static_cast<unsigned long long>(k) * (k - 1) / 2; };
+  unsigned long long s = pairs(n) * (a / M) + static_cast<unsigned long long>(n) * (b / M);
+  a %= M;
+  uint32_t y = a * n + b % M, m = M;
+  while (y >= m) {  // the sum's lattice points seen along the other axis; a < m here
+    n = y / m;
+    const uint32_t rest = y - n * m, q = m / a, r = rest / a;
+    s += pairs(n) * q + static_cast<unsigned long long>(n) * r;
+    const uint32_t next = m - q * a;
     m = a;
-    a = t;
-    if (m == 0) break;
+    a = next;
+    y = a * n + (rest - r * m);
   }
   return s;
 }
@@ -280,55 +281,74 @@ __device__ __forceinline__ unsigned long long cost_before(const AttnCall& c, con
   uint32_t i0 = 0;
   if (s.off < 0) i0 = static_cast<uint32_t>(-s.off) / tq;
   if (x > i0)
-    w += floor_sum(x - i0, KT, tq, static_cast<uint32_t>(s.off + static_cast<int>((i0 + 1) * tq) + static_cast<int>(KT) - 1));
+    w += floor_sum<KT>(x - i0, tq, static_cast<uint32_t>(s.off + static_cast<int>((i0 + 1) * tq) + static_cast<int>(KT) - 1));
   return w;
 }
 
-// One warp: where unit u of the line lies, as (sequence, head, row tile, key tile), with a border inside a job's fixed
-// cost or near its end moved to the job's own border. (batch, 0, 0, 0) behind the last job.
+// One warp: where the line of work is cut for unit x of `units` (as many as there is work for), as (sequence, head, row
+// tile, key tile); (batch, 0, 0, 0) behind the last job. A border inside a job's fixed cost or near its end moves to the
+// job's own border.
 template <uint32_t KT>
-__device__ void locate(const AttnCall& c, unsigned long long u, uint32_t tq, uint32_t (&at)[4]) {
+__device__ void find_border(const AttnCall& c, uint32_t x, uint32_t units, uint32_t tq, uint32_t (&at)[4]) {
   const uint32_t lane = threadIdx.x & 31u;
-  for (uint32_t b0 = 0; b0 < c.batch; b0 += 32) {
-    const uint32_t b = b0 + lane;
-    unsigned long long w = 0;
-    if (b < c.batch) {
-      const Seq s = load_seq(c, b, tq);
+  Seq s = {};
+  unsigned long long w = 0, all = 0, sum = 0;
+  auto weigh = [&](uint32_t b0) {  // this lane's sequence, and the running sum over the warp
+    w = 0;
+    if (b0 + lane < c.batch) {
+      s = load_seq(c, b0 + lane, tq);
       w = cost_before<KT>(c, s, s.tiles, tq) * c.kv_heads;
     }
-    unsigned long long sum = w;
+    sum = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long t = __shfl_up_sync(kFullMask, sum, o);
       if (lane >= static_cast<unsigned>(o)) sum += t;
     }
-    const unsigned hit = __ballot_sync(kFullMask, sum > u);
-    if (hit == 0) {
-      u -= __shfl_sync(kFullMask, sum, 31);
+    return __shfl_sync(kFullMask, sum, 31);
+  };
+  // the last group is weighed first and the first one last, where it is needed next
+  for (uint32_t b0 = (c.batch - 1) / 32 * 32;; b0 -= 32) {
+    all += weigh(b0);
+    if (b0 == 0) break;
+  }
+  at[0] = c.batch, at[1] = at[2] = at[3] = 0;
+  const unsigned long long most = (all + kMinShare - 1) / kMinShare;
+  const uint32_t n = most < units ? static_cast<uint32_t>(most) : units;
+  if (x >= n) return;
+  unsigned long long u = all / n * x + all % n * x / n;
+  for (uint32_t b0 = 0; b0 < c.batch; b0 += 32) {
+    const unsigned long long here = b0 ? weigh(b0) : __shfl_sync(kFullMask, sum, 31);
+    if (u >= here) {
+      u -= here;
       continue;
     }
-    const int src = __ffs(hit) - 1;
+    const int src = __ffs(__ballot_sync(kFullMask, sum > u)) - 1;
     const uint32_t bb = b0 + static_cast<uint32_t>(src);
-    const unsigned long long per_seq = __shfl_sync(kFullMask, w, src);
+    const unsigned long long per_head = __shfl_sync(kFullMask, w, src) / c.kv_heads;
     unsigned long long rest = u - __shfl_sync(kFullMask, sum - w, src);
-    const Seq s = load_seq(c, bb, tq);
-    const unsigned long long per_head = per_seq / c.kv_heads;
-    uint32_t h = static_cast<uint32_t>(rest / per_head);
-    rest -= per_head * h;
+    s.row0 = __shfl_sync(kFullMask, s.row0, src);
+    s.rows = __shfl_sync(kFullMask, s.rows, src);
+    s.len = __shfl_sync(kFullMask, s.len, src);
+    s.off = __shfl_sync(kFullMask, s.off, src);
+    s.tiles = __shfl_sync(kFullMask, s.tiles, src);
+    uint32_t h = 0;
+    while (h + 1 < c.kv_heads && rest >= per_head) rest -= per_head, ++h;
     uint32_t lo = 0, hi = s.tiles;  // cost_before(lo) <= rest < cost_before(hi)
+    unsigned long long before = 0;
     while (hi - lo > 1) {
-      const uint32_t span = hi - lo, step = (span + 31) / 32, mid = lo + step * (lane + 1);
-      const bool over = mid >= hi || cost_before<KT>(c, s, mid, tq) > rest;
-      const int f = __ffs(__ballot_sync(kFullMask, over)) - 1;  // the last lane is always over
-      const uint32_t nlo = lo + step * static_cast<uint32_t>(f), nhi = min(hi, nlo + step);
-      lo = nlo;
-      hi = nhi;
+      const uint32_t step = (hi - lo + 31) / 32, mid = lo + step * (lane + 1);
+      const unsigned long long cost = mid < hi ? cost_before<KT>(c, s, mid, tq) : ~0ull;
+      const int f = __ffs(__ballot_sync(kFullMask, cost > rest)) - 1;  // the last lane's always is
+      if (f > 0) before = __shfl_sync(kFullMask, cost, f - 1);
+      lo += step * static_cast<uint32_t>(f);
+      hi = min(hi, lo + step);
     }
     uint32_t i = lo;
-    rest -= cost_before<KT>(c, s, i, tq);
-    const uint32_t n = (key_end(c, s, i, tq) + KT - 1) / KT;
+    rest -= before;
+    const uint32_t n_keys = (key_end(c, s, i, tq) + KT - 1) / KT;
     uint32_t t = rest <= kJobCost ? 0u : static_cast<uint32_t>(rest) - kJobCost;
-    if (t > 0 && t + kSnap >= n) {
+    if (t > 0 && t + kSnap >= n_keys) {
       t = 0;
       if (++i == s.tiles) {
         i = 0;
@@ -337,7 +357,7 @@ __device__ void locate(const AttnCall& c, unsigned long long u, uint32_t tq, uin
           // the next sequence that has rows
           uint32_t nb = bb + 1;
           while (nb < c.batch && load_seq(c, nb, tq).rows == 0) ++nb;
-          at[0] = nb, at[1] = at[2] = at[3] = 0;
+          at[0] = nb;
           return;
         }
       }
@@ -345,7 +365,6 @@ __device__ void locate(const AttnCall& c, unsigned long long u, uint32_t tq, uin
     at[0] = bb, at[1] = h, at[2] = i, at[3] = t;
     return;
   }
-  at[0] = c.batch, at[1] = at[2] = at[3] = 0;
 }
 
 // The pieces of jobs between two borders, one after the other.
@@ -414,6 +433,25 @@ __device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// The 4 x 4 exchange among four neighbouring lanes: u[j] becomes part (lane & 3) of lane (lane & ~3) + j.
+__device__ __forceinline__ void trade4(uint4 (&u)[4], uint32_t lane) {
+#pragma unroll
+  for (uint32_t bit = 1; bit <= 2; bit <<= 1) {
+    const bool up = (lane & bit) != 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      if (i & bit) continue;
+      uint4 t = up ? u[i] : u[i + bit];
+      t.x = __shfl_xor_sync(kFullMask, t.x, bit);
+      t.y = __shfl_xor_sync(kFullMask, t.y, bit);
+      t.z = __shfl_xor_sync(kFullMask, t.z, bit);
+      t.w = __shfl_xor_sync(kFullMask, t.w, bit);
+      if (up) u[i] = t;
+      else u[i + bit] = t;
+    }
+  }
+}
+
 template <typename T, int D, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ CUtensorMap qmap,
@@ -454,21 +492,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
+  if (threadIdx.x < 3) {
+    const CUtensorMap* map = threadIdx.x == 0 ? &qmap : threadIdx.x == 1 ? &kmap : &vmap;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   pdl_wait_and_trigger();
   if (warp < 2) {
-    // all of the work, and this unit's borders (warp 0 the first, warp 1 the last)
-    unsigned long long w = 0;
-    for (uint32_t b = lane; b < c.batch; b += 32) {
-      const Seq s = load_seq(c, b, tq);
-      w += cost_before<KT>(c, s, s.tiles, tq) * c.kv_heads;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
-    const unsigned long long most = (w + kMinShare - 1) / kMinShare;
-    const uint32_t n = static_cast<uint32_t>(min(static_cast<unsigned long long>(units), most ? most : 1ull));
-    const uint32_t x = unit + warp;
-    uint32_t at[4] = {c.batch, 0, 0, 0};
-    if (x < n) locate<KT>(c, w / n * x + w % n * x / n, tq, at);
+    // this unit's borders: warp 0 finds the first, warp 1 the last
+    uint32_t at[4];
+    find_border<KT>(c, unit + warp, units, tq, at);
     if (lane < 4) (warp ? sh.end : sh.start)[lane] = lane == 0 ? at[0] : lane == 1 ? at[1] : lane == 2 ? at[2] : at[3];
   }
   tc_before();
@@ -506,13 +538,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_4d(base + (ch * most + x * c.box_rows) * 128u, map, static_cast<int>(col + ch * 64), row, static_cast<int>(h), page, &sh.kv_full[st]);
         }
       };
-      // order of use: K(0), K(1), V(0), K(2), V(1), ...
+      // order of use in a job: K(0), K(1), V(0), K(2), V(1), ...
       uint32_t pb = 0, ph = 0, pt = 0, pkeys = 0;
       Seq ps = {};
       for (; pc.next() && !aborted(sh); pc.advance()) {
         for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
-          const uint32_t kslot = fill++;
-          if (g > 0) load_kv(&vmap, ps, pb, ph, pt * KT, KT, pkeys, rank * (D / CG), Sh::kVChunks, fill++);
+          // the stages are used in this order, whichever is asked for first: K(g) ahead of V(g - 1), but behind it at
+          // the start of a job, whose Q can only be copied once the last job's products with Q are done
+          const bool k_ahead = t > pc.t0 && g > 0;
+          const uint32_t kslot = fill + (k_ahead || g == 0 ? 0u : 1u), vslot = fill + (k_ahead ? 1u : 0u);
+          fill += g > 0 ? 2u : 1u;
+          if (g > 0) load_kv(&vmap, ps, pb, ph, pt * KT, KT, pkeys, rank * (D / CG), Sh::kVChunks, vslot);
           if (t == pc.t0) {
             if (job > 0) wait(sh, &sh.q_empty, (job - 1) & 1u);
             if (aborted(sh)) break;
@@ -583,6 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; pc.next() && !aborted(sh); pc.advance()) {
         const uint32_t t0 = uniform(pc.t0), t1 = uniform(pc.t1);
         for (uint32_t t = t0; t < t1; ++t, ++g) {
+          if (t == t0 && g > 0) pv(g - 1);
           const uint32_t buf = uniform(g & 1u);
           const uint64_t qd = smem_desc(qs, 16), d = smem_desc(kvs + uniform(st) * Sh::kStageBytes, 16);
           if (t == t0) wait(sh, &sh.q_full, job & 1u);
@@ -598,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
           next_stage();
-          if (g > 0) pv(g - 1);
+          if (t > t0) pv(g - 1);
           first = t == t0;
           tail = pc.keys - t * KT < KT;
           prev_job = job;
@@ -634,6 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       for (; pc.next() && !aborted(sh); pc.advance()) {
         for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
+          if (t == pc.t0 && g > 0) v_stage();
           if (rank) {
             if (t == pc.t0) {
               wait(sh, &sh.q_full, jobs++ & 1u);
@@ -644,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
           }
           next_stage();
-          if (g > 0) v_stage();
+          if (t > pc.t0) v_stage();
           valid = min(KT, pc.keys - t * KT);
         }
       }
@@ -783,6 +821,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
       constexpr uint32_t kHalf = D / 2;  // columns of a group
       if (busy) {
+        T* out4[4];  // where the rows of this lane's four go; null: no row
+        {
+          T* to = mine ? static_cast<T*>(c.out) + token * c.out_row + (pc.h * c.group + my_head) * c.out_head : nullptr;
+#pragma unroll
+          for (uint32_t y = 0; y < 4; ++y)
+            out4[y] = reinterpret_cast<T*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(to), (lane & ~3u) + y));
+        }
         float* piece = nullptr;
         if (!whole) piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
 #pragma unroll 1
@@ -797,20 +842,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = 0.0f;
           }
-          if (!mine) continue;
           if (whole) {
-            T* to = static_cast<T*>(c.out) + token * c.out_row + (pc.h * c.group + my_head) * c.out_head;
+            // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
+            // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
+            uint4 u[4];
 #pragma unroll
-            for (uint32_t y = 0; y < 32; y += 8)
-              if (col + y < c.dim) {
-                uint4 u;
-                u.x = pack2<T>(__fmul_rn(o[y], inv), __fmul_rn(o[y + 1], inv));
-                u.y = pack2<T>(__fmul_rn(o[y + 2], inv), __fmul_rn(o[y + 3], inv));
-                u.z = pack2<T>(__fmul_rn(o[y + 4], inv), __fmul_rn(o[y + 5], inv));
-                u.w = pack2<T>(__fmul_rn(o[y + 6], inv), __fmul_rn(o[y + 7], inv));
-                *reinterpret_cast<uint4*>(to + col + y) = u;
-              }
-          } else {
+            for (uint32_t y = 0; y < 4; ++y) {
+              u[y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
+              u[y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
+              u[y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
+              u[y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
+            }
+            trade4(u, lane);
+            const uint32_t at = col + (lane & 3u) * 8u;
+            if (at < c.dim) {
+#pragma unroll
+              for (uint32_t y = 0; y < 4; ++y)
+                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
+            }
+          } else if (mine) {
             // [column / 4][row] quads, so that a warp's rows lie side by side
 #pragma unroll
             for (uint32_t y = 0; y < 32; y += 4)
