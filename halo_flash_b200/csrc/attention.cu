@@ -80,16 +80,16 @@ __device__ __forceinline__ void bar_init(unsigned long long* b, uint32_t n) {
 __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
 }
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, unsigned long long* bar) {
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, unsigned long long* bar) {
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -433,6 +433,11 @@ __device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+template <uint32_t V>
+struct Int {
+  static constexpr uint32_t value = V;
+};
+
 // The 4 x 4 exchange among four neighbouring lanes: u[j] becomes part (lane & 3) of lane (lane & ~3) + j.
 __device__ __forceinline__ void trade4(uint4 (&u)[4], uint32_t lane) {
 #pragma unroll
@@ -511,36 +516,47 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     Pieces<KT> pc(c, sh, tq);
-    if (warp == 8 && lane == 0) {
+    if (warp == 8) {
       // ---- copies -------------------------------------------------------------------------------------------------
       uint32_t g = 0, fill = 0, job = 0;
       uint32_t issued = 0;  // stages that have had a load
       const uint32_t q_bytes = tq_cta * c.group * 128u * kChunks;
-      // One operand's tile: `rows` key rows from `key0` on, chunks of 64 columns from `col` on, laid out [chunk][row].
-      auto load_kv = [&](const CUtensorMap* map, const Seq& s, uint32_t b, uint32_t h, uint32_t key0, uint32_t most, uint32_t keys, uint32_t col,
-                         uint32_t chunks, uint32_t seq) {
-        const uint32_t st = seq % ST;
+      // One operand's tile: up to `kMost` key rows from key0 on, kCh chunks of 64 columns from `col` on, laid out
+      // [chunk][row]. One lane looks up each box's page; an elected thread issues the copies.
+      auto load_kv = [&](auto most, auto chunks, const CUtensorMap* map, uint32_t row0, uint32_t b, uint32_t h, uint32_t key0, uint32_t keys,
+                         uint32_t col, uint32_t seq) {
+        constexpr uint32_t kMost = decltype(most)::value, kCh = decltype(chunks)::value;
+        const uint32_t st = uniform(seq % ST);
+        // rows behind the last visible key are left out by whole boxes
+        const uint32_t rows = keys > key0 ? min(kMost, keys - key0) : 0u, box = c.box_rows;
+        const uint32_t boxes = uniform((rows + box - 1) / box);
+        uint32_t page = 0, row = row0 + key0 + lane * box;
+        if (c.table && lane < boxes) {
+          const uint32_t key = key0 + lane * box;
+          page = static_cast<uint32_t>(c.table[b * c.table_stride + (key >> c.page_shift)]);
+          row = key & ((1u << c.page_shift) - 1u);
+        }
         if (seq >= ST) wait(sh, &sh.kv_empty[st], (seq / ST - 1) & 1u);
         if (aborted(sh)) return;
-        const uint32_t base = kv_smem + st * Sh::kStageBytes;
-        // rows behind the last visible key are left out by whole boxes
-        const uint32_t rows = keys > key0 ? min(most, keys - key0) : 0u, boxes = (rows + c.box_rows - 1) / c.box_rows;
-        stage_expect(smem_addr(&sh.kv_full[st]), boxes * c.box_rows * 128u * chunks);
         issued |= 1u << st;
+        const uint32_t bar = uniform(smem_addr(&sh.kv_full[st])), base = uniform(kv_smem + st * Sh::kStageBytes);
+        const uint32_t hh = uniform(h);
+        if (elect()) stage_expect(bar, boxes * box * 128u * kCh);
+        __syncwarp();
         for (uint32_t x = 0; x < boxes; ++x) {
-          const uint32_t key = key0 + x * c.box_rows;
-          int row = static_cast<int>(s.row0 + key), page = 0;
-          if (c.table) {
-            page = c.table[b * c.table_stride + (key >> c.page_shift)];
-            row = static_cast<int>(key & ((1u << c.page_shift) - 1u));
+          const uint32_t r = __shfl_sync(kFullMask, row, x), pg = __shfl_sync(kFullMask, page, x), to = base + uniform(x * box * 128u);
+          if (elect()) {
+#pragma unroll
+            for (uint32_t ch = 0; ch < kCh; ++ch)
+              tma_4d(to + ch * kMost * 128u, map, static_cast<int>(col + ch * 64), static_cast<int>(r), static_cast<int>(hh), static_cast<int>(pg), bar);
           }
-          for (uint32_t ch = 0; ch < chunks; ++ch)
-            tma_4d(base + (ch * most + x * c.box_rows) * 128u, map, static_cast<int>(col + ch * 64), row, static_cast<int>(h), page, &sh.kv_full[st]);
+          __syncwarp();
         }
       };
       // order of use in a job: K(0), K(1), V(0), K(2), V(1), ...
-      uint32_t pb = 0, ph = 0, pt = 0, pkeys = 0;
-      Seq ps = {};
+      uint32_t pb = 0, ph = 0, pt = 0, pkeys = 0, prow = 0;
+      const uint32_t vcol = uniform(rank * (D / CG));
+      auto load_v = [&](uint32_t slot) { load_kv(Int<KT>{}, Int<Sh::kVChunks>{}, &vmap, prow, pb, ph, pt * KT, pkeys, vcol, slot); };
       for (; pc.next() && !aborted(sh); pc.advance()) {
         for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
           // the stages are used in this order, whichever is asked for first: K(g) ahead of V(g - 1), but behind it at
@@ -548,21 +564,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool k_ahead = t > pc.t0 && g > 0;
           const uint32_t kslot = fill + (k_ahead || g == 0 ? 0u : 1u), vslot = fill + (k_ahead ? 1u : 0u);
           fill += g > 0 ? 2u : 1u;
-          if (g > 0) load_kv(&vmap, ps, pb, ph, pt * KT, KT, pkeys, rank * (D / CG), Sh::kVChunks, vslot);
+          if (g > 0) load_v(vslot);
           if (t == pc.t0) {
             if (job > 0) wait(sh, &sh.q_empty, (job - 1) & 1u);
             if (aborted(sh)) break;
-            stage_expect(smem_addr(&sh.q_full), q_bytes);
-            for (uint32_t ch = 0; ch < kChunks; ++ch)
-              tma_3d(q_smem + ch * kRows * 128u, &qmap, static_cast<int>(ch * 64), static_cast<int>(pc.h * c.group),
-                     static_cast<int>(pc.s.row0 + pc.i * tq + rank * tq_cta), &sh.q_full);
+            const uint32_t bar = uniform(smem_addr(&sh.q_full)), head = uniform(pc.h * c.group), tok = uniform(pc.s.row0 + pc.i * tq + rank * tq_cta);
+            const uint32_t to = uniform(q_smem);
+            if (elect()) {
+              stage_expect(bar, q_bytes);
+#pragma unroll
+              for (uint32_t ch = 0; ch < kChunks; ++ch)
+                tma_3d(to + ch * kRows * 128u, &qmap, static_cast<int>(ch * 64), static_cast<int>(head), static_cast<int>(tok), bar);
+            }
+            __syncwarp();
             ++job;
           }
-          load_kv(&kmap, pc.s, pc.b, pc.h, t * KT + rank * Sh::kKeyRows, Sh::kKeyRows, pc.keys, 0, kChunks, kslot);
-          ps = pc.s, pb = pc.b, ph = pc.h, pt = t, pkeys = pc.keys;
+          load_kv(Int<Sh::kKeyRows>{}, Int<kChunks>{}, &kmap, pc.s.row0, pc.b, pc.h, t * KT + rank * Sh::kKeyRows, pc.keys, 0, kslot);
+          prow = pc.s.row0, pb = pc.b, ph = pc.h, pt = t, pkeys = pc.keys;
         }
       }
-      if (g > 0 && !aborted(sh)) load_kv(&vmap, ps, pb, ph, pt * KT, KT, pkeys, rank * (D / CG), Sh::kVChunks, fill++);
+      if (g > 0 && !aborted(sh)) load_v(fill++);
       // every stage's last use is over before the CTA may leave: no arrival of the other CTA's products is under way
       if (!aborted(sh)) {
         for (uint32_t i = fill > ST ? fill - ST : 0u; i < fill; ++i) wait(sh, &sh.kv_empty[i % ST], (i / ST) & 1u);
