@@ -61,7 +61,7 @@ struct Shape {
 };
 
 struct alignas(16) Shared {
-  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty, v_dirty, v_clean, m_full[2][4];
+  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty, v_dirty, v_clean, m_full[2][4], l_full[2][4];
   uint32_t tmem, abort;
   uint32_t start[4], end[4];  // (sequence, K/V head, row tile, key tile) of the piece's borders
   float m[2][kRows];
@@ -478,12 +478,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(&sh.q_empty, 1);
     bar_init(&sh.v_dirty, 1);
     bar_init(&sh.v_clean, 1);
-    bar_init(&sh.o_empty, 8 * CG);
+    bar_init(&sh.o_empty, 4 * CG);
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.s_full[i], 1);
       for (int w = 0; w < 2; ++w) bar_init(&sh.p_full[i][w], 4 * CG);
       bar_init(&sh.pv_done[i], 1);
-      for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1);
+      for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1), bar_init(&sh.l_full[i][w], 1);
     }
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t wg = warp >> 2, quad = warp & 3u, row = quad * 32u + lane;
     const uint32_t lane_base = (quad * 32u) << 16;
     const uint32_t my_tok = row / c.group, my_head = row - my_tok * c.group;
-    uint32_t g = 0;
+    uint32_t g = 0, shares = 0;  // tiles so far, jobs in which both groups had a tile
     if (threadIdx.x == 0 && rank == 0) c.meta[8u * unit] = c.meta[8u * unit + 1] = 0;
     for (; pc.next(); pc.advance()) {
       const uint32_t tok0 = pc.i * tq + rank * tq_cta;
@@ -731,6 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (c.causal) limit = static_cast<uint32_t>(max(0, min(static_cast<int>(pc.keys), pc.s.off + static_cast<int>(tok0 + my_tok) + 1)));
       const uint32_t all_see = c.causal ? static_cast<uint32_t>(max(0, pc.s.off + static_cast<int>(tok0) + 1)) : pc.keys;
       float m = -INFINITY, l = 0.0f;  // the reference that l is relative to
+      float before = -INFINITY;       // the one of the tile before
       for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
         const uint32_t buf = g & 1u;
         if (buf != wg) continue;
@@ -757,6 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             wait(sh, &sh.m_full[buf ^ 1u][quad], ((g - 1) >> 1) & 1u);
             ref = sh.m[buf ^ 1u][row];
           }
+          before = ref;
           // the reference follows where it has fallen too far behind
           const float grown = __fmul_rn(mx - ref, c.scale_log2);
           const bool follow = grown > kLazy;  // also from -inf; false for -inf against -inf (NaN)
@@ -820,91 +822,107 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) tell_leader(&sh.p_full[buf][Sh::kParts - 1]);
       }
-      // the two groups' denominators over one reference, the last tile's
-      const bool any = pc.t1 > pc.t0;
-      float ref = m;
-      if (any && ((g - 1) & 1u) != wg) {
-        wait(sh, &sh.m_full[(g - 1) & 1u][quad], ((g - 1) >> 1) & 1u);
-        ref = sh.m[(g - 1) & 1u][row];
-        if (!busy) ref = -INFINITY;
-        if (m != -INFINITY && ref != m) l = __fmul_rn(l, ex2_approx(__fmul_rn(m - ref, c.scale_log2)));
-      }
-      sh.l[wg][row] = l;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const float total = sh.l[0][row] + sh.l[1][row];
-      const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
-      if (any) {
-        wait(sh, &sh.pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u);
-        tc_after();
-      }
-      const bool mine = row < rows && !aborted(sh);
-      const uint64_t token = pc.s.row0 + tok0 + my_tok;
-      const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-      constexpr uint32_t kHalf = D / 2;  // columns of a group
-      if (busy) {
-        T* out4[4];  // where the rows of this lane's four go; null: no row
-        {
-          T* to = mine ? static_cast<T*>(c.out) + token * c.out_row + (pc.h * c.group + my_head) * c.out_head : nullptr;
+      const bool any = pc.t1 > pc.t0, whole = pc.t0 == 0 && pc.t1 == pc.n;
+      const bool both_groups = pc.t1 - pc.t0 >= 2;
+      const uint32_t shared = shares & 1u, share_phase = (shares >> 1) & 1u;
+      if (both_groups) ++shares;
+      // The group of the last tile writes the outputs, while the other one, having left its denominator behind, goes on
+      // to the next job's first tile.
+      const bool owner = any ? ((g - 1) & 1u) == wg : wg == 0;
+      if (!owner) {
+        if (both_groups) {
+          sh.l[shared][row] = l;
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.l_full[shared][quad]);
+        }
+      } else {
+        const float ref = m;
+        float total = l;
+        if (both_groups) {
+          wait(sh, &sh.l_full[shared][quad], share_phase);
+          // over the reference of the tile before the last one
+          const float other = sh.l[shared][row];
+          if (before == ref) total += other;
+          else if (before != -INFINITY) total = __fmaf_rn(other, ex2_approx(__fmul_rn(before - ref, c.scale_log2)), total);
+        }
+        if (any) {
+          wait(sh, &sh.pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u);
+          tc_after();
+        }
+        const bool mine = row < rows && !aborted(sh);
+        const uint64_t token = pc.s.row0 + tok0 + my_tok;
+        const uint32_t head = pc.h * c.group + my_head;
+        const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+        if (busy && whole) {
+          // All of O is read first, so that the next job's products may start; then the rows are stored.
+          uint4 u[D / 32][4];
+#pragma unroll
+          for (uint32_t x = 0; x < D / 32; ++x) {
+            float o[32];
+            if (any) {
+              tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
+              tc_wait_ld(o);
+            }
+            if (!any || total == 0.0f) {
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+            }
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y) {
+              u[x][y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
+              u[x][y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
+              u[x][y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
+              u[x][y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
+            }
+          }
+          tc_before();
+          __syncwarp();
+          if (any && lane == 0) tell_leader(&sh.o_empty);
+          T* out4[4];  // where the rows of this lane's four go; null: no row
+          T* to = mine ? static_cast<T*>(c.out) + token * c.out_row + head * c.out_head : nullptr;
 #pragma unroll
           for (uint32_t y = 0; y < 4; ++y)
             out4[y] = reinterpret_cast<T*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(to), (lane & ~3u) + y));
-        }
-        float* piece = nullptr;
-        if (!whole) piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
-#pragma unroll 1
-        for (uint32_t x = 0; x < kHalf / 32; ++x) {
-          const uint32_t col = wg * kHalf + x * 32u;
-          float o[32];
-          if (any) {
-            tc_ld32(tmem + lane_base + kTmemO + col, o);
-            tc_wait_ld(o);
-          }
-          if (!any || total == 0.0f) {
+          // A lane holds 64 bytes of its own row at a time; a store of those would touch 32 lines. Four lanes trade their
+          // four 16-byte parts, so that each store covers 64 bytes of each of eight rows.
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-          }
-          if (whole) {
-            // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
-            // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
-            uint4 u[4];
-#pragma unroll
-            for (uint32_t y = 0; y < 4; ++y) {
-              u[y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
-              u[y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
-              u[y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
-              u[y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
-            }
-            trade4(u, lane);
-            const uint32_t at = col + (lane & 3u) * 8u;
+          for (uint32_t x = 0; x < D / 32; ++x) {
+            trade4(u[x], lane);
+            const uint32_t at = x * 32u + (lane & 3u) * 8u;
             if (at < c.dim) {
 #pragma unroll
               for (uint32_t y = 0; y < 4; ++y)
-                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
+                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[x][y];
             }
-          } else if (mine) {
-            // [column / 4][row] quads, so that a warp's rows lie side by side
+          }
+          if (mine && c.lse)
+            c.lse[token * (c.kv_heads * c.group) + head] =
+                total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total)), 0.69314718055994531f);
+        } else {
+          if (busy) {  // a piece of a split job; pieces have tiles
+            float* piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
+#pragma unroll 1
+            for (uint32_t x = 0; x < D / 32; ++x) {
+              float o[32];
+              tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
+              tc_wait_ld(o);
+              // [column / 4][row] quads, so that a warp's rows lie side by side
+              if (mine) {
 #pragma unroll
-            for (uint32_t y = 0; y < 32; y += 4)
-              *reinterpret_cast<float4*>(piece + ((col + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-          }
-        }
-        if (mine && wg == 0) {
-          if (whole) {
-            if (c.lse) {
-              const float lse = total == 0.0f ? -INFINITY
-                                              : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total)), 0.69314718055994531f);
-              c.lse[token * (c.kv_heads * c.group) + pc.h * c.group + my_head] = lse;
+                for (uint32_t y = 0; y < 32; y += 4)
+                  *reinterpret_cast<float4*>(piece + ((x * 32u + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+              }
             }
-          } else {
-            piece[D * kRows + row] = ref;
-            piece[(D + 1) * kRows + row] = total;
+            if (mine) {
+              piece[D * kRows + row] = ref;
+              piece[(D + 1) * kRows + row] = total;
+            }
           }
+          tc_before();
+          __syncwarp();
+          if (any && lane == 0) tell_leader(&sh.o_empty);
         }
       }
-      tc_before();
-      __syncwarp();
-      if (any && lane == 0) tell_leader(&sh.o_empty);
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // before sh.l is written again
       if (threadIdx.x == 0 && rank == 0 && !whole) {
         // what the join needs: a piece that opens a split job says which one, every other one whether it ends it
         uint32_t* to = c.meta + 8u * unit;
