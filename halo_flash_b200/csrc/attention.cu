@@ -676,10 +676,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (rank) wait(sh, &sh.kv_full[st], ph);
         else if (valid < KT) wait(sh, &sh.v_dirty, tails++ & 1u);
         if (valid < KT) {
-          const uint32_t per = (KT - valid) * 8u, base = kv_smem + st * Sh::kStageBytes;
-          for (uint32_t x = lane; x < per * Sh::kVChunks; x += 32) {
-            const uint32_t ch = x / per, at = base + (ch * KT + valid) * 128u + (x - ch * per) * 16u;
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+          const uint32_t base = kv_smem + st * Sh::kStageBytes + lane * 16u;
+#pragma unroll 4
+          for (uint32_t r = valid; r < KT; r += 4) {  // four rows of 128 bytes at a time
+            if (r + lane / 8u < KT) {
+#pragma unroll
+              for (uint32_t ch = 0; ch < Sh::kVChunks; ++ch)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (ch * KT + r) * 128u), "r"(0u) : "memory");
+            }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           if (rank) asm volatile("fence.acq_rel.cluster;" ::: "memory");
@@ -854,9 +858,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t head = pc.h * c.group + my_head;
         const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
         if (busy && whole) {
-          // All of O is read first, so that the next job's products may start; then the rows are stored.
-          uint4 u[D / 32][4];
+          T* out4[4];  // where the rows of this lane's four go; null: no row
+          T* to = mine ? static_cast<T*>(c.out) + token * c.out_row + head * c.out_head : nullptr;
 #pragma unroll
+          for (uint32_t y = 0; y < 4; ++y)
+            out4[y] = reinterpret_cast<T*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(to), (lane & ~3u) + y));
+          // The loop stays rolled: unrolled, its first pass is bound by instruction fetches (10000 cycles for 64 KB).
+#pragma unroll 1
           for (uint32_t x = 0; x < D / 32; ++x) {
             float o[32];
             if (any) {
@@ -867,61 +875,49 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int y = 0; y < 32; ++y) o[y] = 0.0f;
             }
+            uint4 u[4];
 #pragma unroll
             for (uint32_t y = 0; y < 4; ++y) {
-              u[x][y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
-              u[x][y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
-              u[x][y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
-              u[x][y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
+              u[y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
+              u[y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
+              u[y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
+              u[y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
             }
-          }
-          tc_before();
-          __syncwarp();
-          if (any && lane == 0) tell_leader(&sh.o_empty);
-          T* out4[4];  // where the rows of this lane's four go; null: no row
-          T* to = mine ? static_cast<T*>(c.out) + token * c.out_row + head * c.out_head : nullptr;
-#pragma unroll
-          for (uint32_t y = 0; y < 4; ++y)
-            out4[y] = reinterpret_cast<T*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(to), (lane & ~3u) + y));
-          // A lane holds 64 bytes of its own row at a time; a store of those would touch 32 lines. Four lanes trade their
-          // four 16-byte parts, so that each store covers 64 bytes of each of eight rows.
-#pragma unroll
-          for (uint32_t x = 0; x < D / 32; ++x) {
-            trade4(u[x], lane);
+            // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
+            // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
+            trade4(u, lane);
             const uint32_t at = x * 32u + (lane & 3u) * 8u;
             if (at < c.dim) {
 #pragma unroll
               for (uint32_t y = 0; y < 4; ++y)
-                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[x][y];
+                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
             }
           }
           if (mine && c.lse)
             c.lse[token * (c.kv_heads * c.group) + head] =
                 total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total)), 0.69314718055994531f);
-        } else {
-          if (busy) {  // a piece of a split job; pieces have tiles
-            float* piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
+        } else if (busy) {  // a piece of a split job; pieces have tiles
+          float* piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
 #pragma unroll 1
-            for (uint32_t x = 0; x < D / 32; ++x) {
-              float o[32];
-              tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
-              tc_wait_ld(o);
-              // [column / 4][row] quads, so that a warp's rows lie side by side
-              if (mine) {
-#pragma unroll
-                for (uint32_t y = 0; y < 32; y += 4)
-                  *reinterpret_cast<float4*>(piece + ((x * 32u + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-              }
-            }
+          for (uint32_t x = 0; x < D / 32; ++x) {
+            float o[32];
+            tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
+            tc_wait_ld(o);
+            // [column / 4][row] quads, so that a warp's rows lie side by side
             if (mine) {
-              piece[D * kRows + row] = ref;
-              piece[(D + 1) * kRows + row] = total;
+#pragma unroll
+              for (uint32_t y = 0; y < 32; y += 4)
+                *reinterpret_cast<float4*>(piece + ((x * 32u + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
           }
-          tc_before();
-          __syncwarp();
-          if (any && lane == 0) tell_leader(&sh.o_empty);
+          if (mine) {
+            piece[D * kRows + row] = ref;
+            piece[(D + 1) * kRows + row] = total;
+          }
         }
+        tc_before();
+        __syncwarp();
+        if (any && lane == 0) tell_leader(&sh.o_empty);
       }
       if (threadIdx.x == 0 && rank == 0 && !whole) {
         // what the join needs: a piece that opens a split job says which one, every other one whether it ends it
