@@ -750,8 +750,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (key0 + KT > min(all_see, pc.keys)) {
             const uint32_t left = limit > key0 ? limit - key0 : 0u;
 #pragma unroll
-            for (uint32_t x = 0; x < KT; ++x)
-              if (x >= left) s[x / 32][x % 32] = -INFINITY;
+            for (uint32_t x = 0; x < KT / 32; ++x) {
+              const uint32_t over = left > x * 32 ? left - x * 32 : 0u, keep = over >= 32 ? 0xFFFFFFFFu : (1u << over) - 1u;
+#pragma unroll
+              for (uint32_t y = 0; y < 32; ++y)
+                if (!(keep & (1u << y))) s[x][y] = -INFINITY;
+            }
           }
           float mx = -INFINITY;
 #pragma unroll
@@ -865,32 +869,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             out4[y] = reinterpret_cast<T*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(to), (lane & ~3u) + y));
           // The loop stays rolled: unrolled, its first pass is bound by instruction fetches (10000 cycles for 64 KB).
 #pragma unroll 1
-          for (uint32_t x = 0; x < D / 32; ++x) {
-            float o[32];
-            if (any) {
-              tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
-              tc_wait_ld(o);
-            }
-            if (!any || total == 0.0f) {
+          for (uint32_t x = 0; x < D / 32; x += 2) {
+            float o[2][32];
+            tc_ld32(tmem + lane_base + kTmemO + x * 32u, o[0]);
+            tc_ld32(tmem + lane_base + kTmemO + x * 32u + 32u, o[1]);
+            tc_wait_ld(o);
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-            }
-            uint4 u[4];
+            for (uint32_t z = 0; z < 2; ++z) {
+              uint4 u[4];
 #pragma unroll
-            for (uint32_t y = 0; y < 4; ++y) {
-              u[y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
-              u[y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
-              u[y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
-              u[y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
-            }
-            // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
-            // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
-            trade4(u, lane);
-            const uint32_t at = x * 32u + (lane & 3u) * 8u;
-            if (at < c.dim) {
+              for (uint32_t y = 0; y < 4; ++y) {
+                u[y].x = pack2<T>(__fmul_rn(o[z][8 * y], inv), __fmul_rn(o[z][8 * y + 1], inv));
+                u[y].y = pack2<T>(__fmul_rn(o[z][8 * y + 2], inv), __fmul_rn(o[z][8 * y + 3], inv));
+                u[y].z = pack2<T>(__fmul_rn(o[z][8 * y + 4], inv), __fmul_rn(o[z][8 * y + 5], inv));
+                u[y].w = pack2<T>(__fmul_rn(o[z][8 * y + 6], inv), __fmul_rn(o[z][8 * y + 7], inv));
+                if (total == 0.0f) u[y] = make_uint4(0, 0, 0, 0);  // no key (and without tiles O holds anything)
+              }
+              // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
+              // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
+              trade4(u, lane);
+              const uint32_t at = (x + z) * 32u + (lane & 3u) * 8u;
+              if (at < c.dim) {
 #pragma unroll
-              for (uint32_t y = 0; y < 4; ++y)
-                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
+                for (uint32_t y = 0; y < 4; ++y)
+                  if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
+              }
             }
           }
           if (mine && c.lse)
