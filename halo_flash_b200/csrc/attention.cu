@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (threadIdx.x == 0 && rank == 0 && !whole) {
         // what the join needs: a piece that opens a split job says which one, every other one whether it ends it
         uint32_t* to = c.meta + 8u * unit;
-        if (pc.t0 == 0) to[1] = 1u, to[2] = pc.b, to[3] = pc.h, to[4] = pc.i;
+        if (pc.t0 == 0) to[1] = 1u, to[2] = pc.s.row0 + pc.i * tq, to[3] = min(tq, pc.s.rows - pc.i * tq), to[4] = pc.h;
         else to[0] = pc.t1 == pc.n ? 2u : 1u;
       }
     }
@@ -944,26 +944,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---- joining the pieces of split jobs -----------------------------------------------------------------------------
 // out = sum_p 2^(c (r_p - R)) O_p / sum_p 2^(c (r_p - R)) l_p over a job's pieces p, R the largest of their references.
-// blockIdx.x: the split job, counted over the CTAs that opened one; blockIdx.y: 32 rows and a share of the columns. Few
-// pieces (a prompt's jobs are cut once): a warp sums a column quad over all of them; many (one token over a long cache
-// is cut by every CTA): the warps share the pieces and meet in shared memory. The order of the sums is fixed.
-constexpr uint32_t kJoinWarps = 8;
+// blockIdx.x: the split job, counted over the units that opened one; blockIdx.y: 32 rows (lane = row) and a share of the
+// columns. What bounds it is latency: a chain of dependent round trips to L2 (flags, then everything else), so all loads
+// of a stage are in flight together. Few pieces (a prompt's jobs are cut once): a warp sums its column quads over all
+// of them and keeps the weights in registers. Many (one token over a long cache is cut by every unit): the warps share
+// the pieces and meet in shared memory. The order of the sums is fixed.
+constexpr uint32_t kJoinResident = 4;  // CTAs on an SM: a grid of one wave (in four waves of two the join of 74 jobs took 17 us)
+constexpr uint32_t kJoinWarps = 8, kFew = 4, kFewQuads = 4, kManyQuads = 2;
 template <typename T, int D, int CG>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnCall c, const uint32_t units) {
-  __shared__ uint32_t opens[(kMaxCtas + 31) / 32], ends[(kMaxCtas + 31) / 32];
-  __shared__ float weight[kMaxCtas + 1][32];
-  __shared__ float4 red[kJoinWarps][32];
+__global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join_kernel(const __grid_constant__ AttnCall c, const uint32_t units) {
+  constexpr uint32_t kWords = (kMaxCtas + 31) / 32;
+  __shared__ uint32_t opens[kWords], ends[kWords];
+  __shared__ float meet[kJoinWarps][32];
+  __shared__ float4 red[kJoinWarps][kManyQuads][32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   pdl_wait_and_trigger();
-  if (warp < (kMaxCtas + 31) / 32) {
+  if (warp < kWords) {
     const uint32_t x = warp * 32u + lane;
-    const uint32_t f0 = x < units ? c.meta[8u * x] : 0u, f1 = x < units ? c.meta[8u * x + 1] : 0u;
-    const uint32_t o = __ballot_sync(kFullMask, f1 == 1u), e = __ballot_sync(kFullMask, f0 == 2u);
+    const uint2 f = x < units ? *reinterpret_cast<const uint2*>(c.meta + 8u * x) : make_uint2(0, 0);
+    const uint32_t o = __ballot_sync(kFullMask, f.y == 1u), e = __ballot_sync(kFullMask, f.x == 2u);
     if (lane == 0) opens[warp] = o, ends[warp] = e;
   }
   __syncthreads();
   uint32_t k = blockIdx.x, first = kMaxCtas;
-  for (uint32_t w = 0; w < (kMaxCtas + 31) / 32; ++w) {
+  for (uint32_t w = 0; w < kWords; ++w) {
     const uint32_t n = __popc(opens[w]);
     if (k < n) {
       uint32_t v = opens[w];
@@ -975,7 +979,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
   }
   if (first >= units) return;
   uint32_t last = first;
-  for (uint32_t w = (first + 1) / 32; w < (kMaxCtas + 31) / 32; ++w) {
+  for (uint32_t w = (first + 1) / 32; w < kWords; ++w) {
     uint32_t v = ends[w];
     if (w == (first + 1) / 32) v &= ~0u << ((first + 1) & 31u);
     if (v) {
@@ -984,77 +988,134 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
     }
   }
   const uint32_t pieces = last - first + 1;
-  const uint32_t* job = c.meta + 8u * first;
-  const uint32_t tq_cta = kRows / c.group, group = blockIdx.y % (4 * CG), rank = group >> 2;
-  const uint32_t h = job[3], tok0 = job[4] * CG * tq_cta + rank * tq_cta;
-  const Seq s = load_seq(c, job[2], CG * tq_cta);
-  const uint32_t rows = tok0 < s.rows ? min(tq_cta, s.rows - tok0) * c.group : 0u;
-  const uint32_t row = (group & 3u) * 32u + lane;
-  if ((group & 3u) * 32u >= rows) return;
-  // piece 0 opened the job, the others are what the CTAs behind began with
+  const uint32_t group = blockIdx.y % (4 * CG), rank = group >> 2, row = (group & 3u) * 32u + lane;
+  // piece 0 opened the job, the others are what the units behind began with
   auto piece = [&](uint32_t p) { return c.part + ((2ull * (first + p) + (p == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D); };
-  for (uint32_t p = warp; p < pieces; p += kJoinWarps) weight[p][lane] = row < rows ? piece(p)[D * kRows + row] : -INFINITY;
-  __syncthreads();
-  float top = -INFINITY;
-  for (uint32_t p = 0; p < pieces; ++p) top = fmaxf(top, weight[p][lane]);
-  __syncthreads();
-  for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
-    const float r = weight[p][lane];
-    weight[p][lane] = r == -INFINITY ? 0.0f : ex2_approx(__fmul_rn(r - top, c.scale_log2));
-  }
-  __syncthreads();
-  float total = 0.0f;
-  for (uint32_t p = warp; p < pieces; p += kJoinWarps)
-    if (row < rows) {
-      const float w = weight[p][lane];
-      if (w != 0.0f) total = __fmaf_rn(w, piece(p)[(D + 1) * kRows + row], total);
+  const uint4 job = *reinterpret_cast<const uint4*>(c.meta + 8u * first);  // ., ., first token, tokens
+  const uint32_t h = c.meta[8u * first + 4];
+  const uint32_t tq_cta = kRows / c.group, tok0 = rank * tq_cta;
+  const uint32_t rows = tok0 < job.w ? min(tq_cta, job.w - tok0) * c.group : 0u;
+  if ((group & 3u) * 32u >= rows) return;
+  const bool mine = row < rows;
+  const uint64_t token = job.z + tok0 + row / c.group;
+  const uint32_t head = h * c.group + row % c.group;
+  T* out = static_cast<T*>(c.out) + token * c.out_row + head * c.out_head;
+  const uint32_t parts = gridDim.y / (4 * CG), quads = D / 4 / parts, q0 = blockIdx.y / (4 * CG) * quads;
+  auto finish2 = [&](uint32_t q, const float4 (&sum)[2], float inv) {  // two quads, q even
+    if (mine && q * 4 < c.dim) {
+      uint4 u;
+      u.x = pack2<T>(__fmul_rn(sum[0].x, inv), __fmul_rn(sum[0].y, inv));
+      u.y = pack2<T>(__fmul_rn(sum[0].z, inv), __fmul_rn(sum[0].w, inv));
+      u.z = pack2<T>(__fmul_rn(sum[1].x, inv), __fmul_rn(sum[1].y, inv));
+      u.w = pack2<T>(__fmul_rn(sum[1].z, inv), __fmul_rn(sum[1].w, inv));
+      *reinterpret_cast<uint4*>(out + q * 4) = u;
     }
-  red[warp][lane].x = total;
+  };
+  auto finish_lse = [&](float top, float total) {
+    if (c.lse && blockIdx.y < 4 * CG && warp == 0 && mine)
+      c.lse[token * (c.kv_heads * c.group) + head] =
+          total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total)), 0.69314718055994531f);
+  };
+  // a piece that saw nothing (weight 0) says nothing, whatever its sums are
+  auto add = [](float4& sum, float w, float4 v) {
+    if (w != 0.0f) {
+      sum.x = __fmaf_rn(w, v.x, sum.x);
+      sum.y = __fmaf_rn(w, v.y, sum.y);
+      sum.z = __fmaf_rn(w, v.z, sum.z);
+      sum.w = __fmaf_rn(w, v.w, sum.w);
+    }
+  };
+  auto quad = [&](uint32_t p, uint32_t q) { return *reinterpret_cast<const float4*>(piece(p) + (q * kRows + row) * 4); };
+  auto weight = [&](float r, float top) { return r == -INFINITY ? 0.0f : ex2_approx(__fmul_rn(r - top, c.scale_log2)); };
+
+  if (pieces <= kFew) {
+    float r[kFew], l[kFew], top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (uint32_t p = 0; p < kFew; ++p) {
+      r[p] = mine && p < pieces ? piece(p)[D * kRows + row] : -INFINITY;
+      l[p] = mine && p < pieces ? piece(p)[(D + 1) * kRows + row] : 0.0f;
+    }
+    // Two pieces are by far the most common: their loads do not wait for the weights. A warp takes four neighbouring
+    // quads, so that a lane's 16 values fill a 32-byte sector of the output.
+    for (uint32_t q = q0 + warp * kFewQuads; q < q0 + quads; q += kJoinWarps * kFewQuads) {
+      float4 v[2][kFewQuads];
+#pragma unroll
+      for (uint32_t x = 0; x < kFewQuads; ++x)
+#pragma unroll
+        for (uint32_t p = 0; p < 2; ++p) v[p][x] = mine ? quad(p, q + x) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (q == q0 + warp * kFewQuads) {
+#pragma unroll
+        for (uint32_t p = 0; p < kFew; ++p) top = fmaxf(top, r[p]);
+#pragma unroll
+        for (uint32_t p = 0; p < kFew; ++p) {
+          r[p] = weight(r[p], top);
+          if (r[p] != 0.0f) total = __fmaf_rn(r[p], l[p], total);
+        }
+      }
+      const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+#pragma unroll
+      for (uint32_t x = 0; x < kFewQuads; x += 2) {
+        float4 sum[2] = {};
+#pragma unroll
+        for (uint32_t y = 0; y < 2; ++y) {
+          add(sum[y], r[0], v[0][x + y]);
+          add(sum[y], r[1], v[1][x + y]);
+          if (mine && pieces > 2) add(sum[y], r[2], quad(2, q + x + y));
+          if (mine && pieces > 3) add(sum[y], r[3], quad(3, q + x + y));
+        }
+        finish2(q + x, sum, inv);
+      }
+    }
+    finish_lse(top, total);
+    return;
+  }
+
+  // each warp over its pieces, then all warps over the warps
+  auto ref = [&](uint32_t p) { return mine ? piece(p)[D * kRows + row] : -INFINITY; };
+  float top = -INFINITY, total = 0.0f;
+#pragma unroll 4
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps) top = fmaxf(top, ref(p));
+  meet[warp][lane] = top;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t w = 0; w < kJoinWarps; ++w) top = fmaxf(top, meet[w][lane]);
+  __syncthreads();
+#pragma unroll 4
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
+    const float w = weight(ref(p), top);
+    if (w != 0.0f) total = __fmaf_rn(w, piece(p)[(D + 1) * kRows + row], total);
+  }
+  meet[warp][lane] = total;
   __syncthreads();
   total = 0.0f;
 #pragma unroll
-  for (uint32_t w = 0; w < kJoinWarps; ++w) total += red[w][lane].x;
-  __syncthreads();
+  for (uint32_t w = 0; w < kJoinWarps; ++w) total += meet[w][lane];
   const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-  const uint64_t token = s.row0 + tok0 + row / c.group;
-  const uint32_t head = h * c.group + row % c.group;
-  T* out = static_cast<T*>(c.out) + token * c.out_row + head * c.out_head;
-  if (c.lse && blockIdx.y < 4 * CG && warp == 0 && row < rows)
-    c.lse[token * (c.kv_heads * c.group) + head] =
-        total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total)), 0.69314718055994531f);
-  const bool shared = pieces > 4;
-  const uint32_t p0 = shared ? warp : 0u, pstep = shared ? kJoinWarps : 1u;
-  const uint32_t parts = gridDim.y / (4 * CG), quads = D / 4 / parts, q0 = blockIdx.y / (4 * CG) * quads;
-  for (uint32_t q = q0 + (shared ? 0u : warp); q < q0 + quads; q += shared ? 1u : kJoinWarps) {
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (row < rows) {
-#pragma unroll 4
-      for (uint32_t p = p0; p < pieces; p += pstep) {
-        const float4 v = *reinterpret_cast<const float4*>(piece(p) + (q * kRows + row) * 4);
-        const float w = weight[p][lane];
-        if (w != 0.0f) {  // a piece that saw nothing says nothing
-          sum.x = __fmaf_rn(w, v.x, sum.x);
-          sum.y = __fmaf_rn(w, v.y, sum.y);
-          sum.z = __fmaf_rn(w, v.z, sum.z);
-          sum.w = __fmaf_rn(w, v.w, sum.w);
-        }
-      }
-    }
-    if (shared) {
-      red[warp][lane] = sum;
-      __syncthreads();
-      sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (warp == 0) {
+  finish_lse(top, total);
+  for (uint32_t q = q0; q < q0 + quads; q += kManyQuads) {
+    float4 sum[kManyQuads] = {};
+    if (mine) {
+#pragma unroll 3
+      for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
+        const float w = weight(ref(p), top);
 #pragma unroll
-        for (uint32_t w = 0; w < kJoinWarps; ++w) sum.x += red[w][lane].x, sum.y += red[w][lane].y, sum.z += red[w][lane].z, sum.w += red[w][lane].w;
+        for (uint32_t x = 0; x < kManyQuads; ++x) add(sum[x], w, quad(p, q + x));
       }
-      __syncthreads();
     }
-    if (row < rows && q * 4 < c.dim && (!shared || warp == 0)) {
-      uint2 u;
-      u.x = pack2<T>(__fmul_rn(sum.x, inv), __fmul_rn(sum.y, inv));
-      u.y = pack2<T>(__fmul_rn(sum.z, inv), __fmul_rn(sum.w, inv));
-      *reinterpret_cast<uint2*>(out + q * 4) = u;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t x = 0; x < kManyQuads; ++x) red[warp][x][lane] = sum[x];
+    __syncthreads();
+    if (warp == 0) {
+      float4 all[2] = {};
+#pragma unroll
+      for (uint32_t w = 0; w < kJoinWarps; ++w)
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x) {
+          const float4 v = red[w][x][lane];
+          all[x].x += v.x, all[x].y += v.y, all[x].z += v.z, all[x].w += v.w;
+        }
+      finish2(q, all, inv);
     }
   }
 }
@@ -1162,7 +1223,7 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   if (e != cudaSuccess || tiles <= 1 || units == 1) return e;
   const uint32_t x = static_cast<uint32_t>(jobs < units ? jobs : units);
   uint32_t parts = 1;
-  while (parts < D / 16 && x * 4 * CG * parts * 2 <= 148 * 8) parts *= 2;
+  while (parts < D / 16 && x * 4 * CG * parts * 2 <= static_cast<uint32_t>(sms) * kJoinResident) parts *= 2;
   return LaunchKernel(attention_join_kernel<T, D, CG>, dim3(x, 4 * CG * parts), kJoinWarps * 32, 0, s, c, static_cast<uint32_t>(units));
 }
 
