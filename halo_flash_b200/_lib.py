@@ -7,6 +7,7 @@ HaloError with the library's own message.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -145,7 +146,8 @@ class Library:
             f = getattr(self.cdll, name)
             f.restype = C.c_int
             f.argtypes = [_p, *mid, C.c_char_p, _sz]
-            self._fn[name] = f
+            self._fn[name[len("halo_b200_"):]] = f
+        self._local = threading.local()  # one message buffer for each thread
         self.cdll.halo_b200_version.restype = C.c_char_p
         self.cdll.halo_b200_version.argtypes = []
         self.cdll.halo_b200_kernel_count.restype = _sz
@@ -173,8 +175,11 @@ class Library:
 
     def call(self, name: str, stream: int, *args) -> None:
         """Invoke `halo_b200_<name>`; raises HaloError with the library's message on failure."""
-        err = C.create_string_buffer(512)
-        rc = self._fn["halo_b200_" + name](stream, *args, err, len(err))
+        try:
+            err = self._local.err
+        except AttributeError:
+            err = self._local.err = C.create_string_buffer(512)
+        rc = self._fn[name](stream, *args, err, 512)
         self.calls += 1
         if rc != 0:
             raise HaloError(err.value.decode(errors="replace"))

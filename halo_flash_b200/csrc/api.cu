@@ -211,8 +211,11 @@ int RunAttention(AttnArgs a, uint64_t workspace_bytes, const char* what, halo_b2
   REQUIRE(Aligned(a.q, 16) && Aligned(a.k, 16) && Aligned(a.v, 16) && Aligned(a.out, 16), "%s: pointer not 16-byte aligned", what);
   REQUIRE(Aligned(a.cu, 4) && Aligned(a.kv_len, 4) && Aligned(a.table, 4) && Aligned(a.lse, 4),
           "%s: pointer not aligned to its element type", what);
-  const uint64_t strides[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.k_page, a.v_row, a.v_head, a.v_page, a.out_row, a.out_head};
-  for (const uint64_t v : strides) REQUIRE(v % 8 == 0 && v < (uint64_t{1} << 38), "%s: strides must be multiples of 8", what);
+  // the stride of an axis with one entry is never used
+  const uint64_t rows = a.table ? 2 : a.tokens;  // a page has 8 rows at least
+  const uint64_t strides[][2] = {{a.q_row, a.tokens}, {a.q_head, a.q_heads},  {a.k_row, rows},      {a.k_head, a.kv_heads}, {a.k_page, a.pages},
+                                 {a.v_row, rows},     {a.v_head, a.kv_heads}, {a.v_page, a.pages},  {a.out_row, a.tokens},  {a.out_head, a.q_heads}};
+  for (const auto& v : strides) REQUIRE(v[1] <= 1 || (v[0] % 8 == 0 && v[0] < (uint64_t{1} << 38)), "%s: strides must be multiples of 8", what);
   REQUIRE(a.workspace && Aligned(a.workspace, 16), "%s: the workspace is null or not 16-byte aligned", what);
   REQUIRE(workspace_bytes >= AttentionWorkspaceBytes(a.dim), "%s: the workspace has %llu bytes, %llu are needed", what,
           static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(AttentionWorkspaceBytes(a.dim)));
@@ -1649,7 +1652,9 @@ int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row
   a.dim = dim;
   a.page_shift = Log2(page_size);
   a.pages = pages;
-  const uint64_t odd = k_row_stride | k_head_stride | v_row_stride | v_head_stride | page_stride | row_stride | head_stride | dim;
+  // strides of axes with one entry are never used
+  const uint64_t odd = (tokens > 1 ? k_row_stride | v_row_stride : 0) | (heads > 1 ? k_head_stride | v_head_stride | head_stride : 0) |
+                       (pages > 1 ? page_stride : 0) | row_stride | dim;
   a.vec = odd % 8 == 0 && Aligned(k, 16) && Aligned(v, 16) && Aligned(k_cache, 16) && Aligned(v_cache, 16);
   const cudaError_t e = LaunchPagedStore(a, S(stream));
   if (e == cudaErrorInvalidValue) return Fail(err, errlen, "%s: unsupported (rows, cache) dtype combination", what);

@@ -17,8 +17,14 @@ from ._lib import BF16, F16, F32, lib
 _DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
+# The raw stream without a Stream object around it (3 us a call); torch's own compiled code asks for it like this.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _chk(t: torch.Tensor | None, name: str, dtypes=None):
@@ -317,53 +323,59 @@ def moe_combine(yp, pos, mw, out, *, sx=None, sg=None):
 
 
 # ---- paged K/V cache and attention ----------------------------------------------------------------
+# A decode step calls these for every layer with a few rows, so what they do on the host is kept short.
 _INT = (torch.int32, torch.uint32)
+_I64 = (torch.int64,)
+_HALF = (torch.float16, torch.bfloat16)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _here(*tensors):
     """The kernels run on the current device's current stream: every tensor must live there."""
+    device = _device()
     for t in tensors:
-        if t is not None and t.device.index != torch.cuda.current_device():
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{device}")
+    return device
 
 
 def _rows(t, name, dtypes, rank=3):
-    """A CUDA tensor of `rank` axes whose last one is contiguous; the other strides are free."""
+    """(shape, strides) of a CUDA tensor of `rank` axes whose last one is contiguous; the other strides are free."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name}: expected a CUDA tensor (halo_flash_b200 has no CPU path)")
-    if t.dim() != rank:
-        raise ValueError(f"{name}: expected {rank} axes, got shape {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: dtype {t.dtype} not in {dtypes}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != rank:
+        raise ValueError(f"{name}: expected {rank} axes, got shape {tuple(shape)}")
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: the last axis must be contiguous")
-    return t
-
-
-def _strides(t, *axes):
-    """Strides in elements; an axis of one entry is never stepped along, whatever torch says its stride is."""
-    return [t.stride(a) if t.shape[a] > 1 else 0 for a in axes]
+    return shape, strides
 
 
 def _caches(k_cache, v_cache, dtypes):
-    _rows(k_cache, "k_cache", dtypes, 4), _rows(v_cache, "v_cache", (k_cache.dtype,), 4)
-    if k_cache.shape != v_cache.shape or _strides(k_cache, 0, 1, 2) != _strides(v_cache, 0, 1, 2):
+    shape, strides = _rows(k_cache, "k_cache", dtypes, 4)
+    v_shape, v_strides = _rows(v_cache, "v_cache", (k_cache.dtype,), 4)
+    if shape != v_shape or (strides != v_strides and any(a != b and n > 1 for a, b, n in zip(strides, v_strides, shape))):
         raise ValueError("k_cache and v_cache must have the same shape and strides")
-    return k_cache.shape
+    return shape, strides
 
 
 def _table(table):
-    _rows(table, "table", _INT, 2)
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+    (rows, cols), (stride, _) = _rows(table, "table", _INT, 2)
+    if rows > 1 and stride < cols:
         raise ValueError("table: rows overlap")
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1]
+    return rows, cols, stride
 
 
-def _vector(t, name, dtypes, n):
+def _vector(t, name, dtypes, n=None):
+    """The address of a contiguous CUDA tensor of n entries, None for None."""
+    if t is None:
+        return None
     _chk(t, name, dtypes)
-    if t is not None and t.numel() != n:
+    if n is not None and t.numel() != n:
         raise ValueError(f"{name}: expected {n} entries, got {t.numel()}")
-    return t
+    return t.data_ptr()
 
 
 def paged_plan(table, past, fresh, free_pages, page_size, slot, *, pos=None, cu=None, kv_len=None, status=None):
@@ -372,27 +384,34 @@ def paged_plan(table, past, fresh, free_pages, page_size, slot, *, pos=None, cu=
     token's page * page_size + offset (-1: refused, or behind the last new token), pos its position, cu [B + 1] the
     prefix sum of fresh, kv_len past + fresh, status [pages taken, requests refused, new tokens]. A request that the
     table row or the free list cannot hold is refused: no pages, slots -1, kv_len = past."""
-    stride, cols = _table(table)
-    batch = table.shape[0]
-    _vector(past, "past", _INT, batch), _vector(fresh, "fresh", _INT, batch), _chk(free_pages, "free_pages", _INT)
-    _chk(slot, "slot", (torch.int64,)), _vector(pos, "pos", _INT, slot.numel()), _vector(cu, "cu", _INT, batch + 1)
-    _vector(kv_len, "kv_len", _INT, batch), _vector(status, "status", _INT, 3)
+    if slot is None or past is None or fresh is None or free_pages is None:
+        raise TypeError("past, fresh, free_pages and slot are needed")
+    batch, cols, stride = _table(table)
+    slots = _vector(slot, "slot", _I64)
+    tokens = slot.numel()
+    args = (table.data_ptr(), stride, cols, _vector(past, "past", _INT, batch), _vector(fresh, "fresh", _INT, batch),
+            _vector(free_pages, "free_pages", _INT), free_pages.numel(), page_size, slots, _vector(pos, "pos", _INT, tokens),
+            _vector(cu, "cu", _INT, batch + 1), _vector(kv_len, "kv_len", _INT, batch), _vector(status, "status", _INT, 3), batch, tokens)
     _here(table, past, fresh, free_pages, slot, pos, cu, kv_len, status)
-    lib().call("paged_plan", _stream(), _p(table), stride, cols, _p(past), _p(fresh), _p(free_pages), free_pages.numel(),
-               page_size, _p(slot), _p(pos), _p(cu), _p(kv_len), _p(status), batch, slot.numel())
+    lib().call("paged_plan", _stream(), *args)
     return slot
 
 
 def paged_store(k, v, k_cache, v_cache, slot):
     """Rows k, v [T, heads, d] to the rows of the caches [pages, page_size, heads, d] that slot (int64 [T]) names;
     slots outside the cache are skipped, and no two of a call may be equal. The caches may be views of any strides."""
-    pages, page_size, heads, d = _caches(k_cache, v_cache, _ACT)
-    _rows(k, "k", _ACT), _rows(v, "v", (k.dtype,)), _vector(slot, "slot", (torch.int64,), k.shape[0])
-    if k.shape != v.shape or tuple(k.shape[1:]) != (heads, d):
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit caches of {heads} heads of {d}")
+    (pages, page_size, heads, d), cs = _caches(k_cache, v_cache, _ACT)
+    shape, ks = _rows(k, "k", _ACT)
+    v_shape, vs = _rows(v, "v", (k.dtype,))
+    tokens = shape[0]
+    if shape != v_shape or shape[1] != heads or shape[2] != d:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v_shape)} do not fit caches of {heads} heads of {d}")
+    if slot is None:
+        raise TypeError("slot is needed")
+    slots = _vector(slot, "slot", _I64, tokens)
     _here(k, v, k_cache, v_cache, slot)
-    lib().call("paged_store", _stream(), _p(k), *_strides(k, 0, 1), _p(v), *_strides(v, 0, 1), _code(k), _p(k_cache),
-               _p(v_cache), _code(k_cache), *_strides(k_cache, 0, 1, 2), pages, page_size, _p(slot), heads, d, k.shape[0])
+    lib().call("paged_store", _stream(), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _DT[k.dtype], k_cache.data_ptr(),
+               v_cache.data_ptr(), _DT[k_cache.dtype], cs[0], cs[1], cs[2], pages, page_size, slots, heads, d, tokens)
 
 
 def attention_workspace(d, device=None):
@@ -401,32 +420,35 @@ def attention_workspace(d, device=None):
     return torch.empty(lib().cdll.halo_b200_attention_workspace(d), dtype=torch.uint8, device=device or "cuda")
 
 
-def _attention(q, out, cu, lse, workspace, scale):
-    _rows(q, "q", (torch.float16, torch.bfloat16)), _rows(out, "out", (q.dtype,)), _chk(cu, "cu", _INT)
-    if out.shape != q.shape:
-        raise ValueError(f"out {tuple(out.shape)} must have the shape of q {tuple(q.shape)}")
-    if cu.numel() < 1:
+def _attention(q, out, cu, lse, workspace):
+    """What both forms check and pass on: (q's shape and strides, out's strides, addresses of cu, lse and the workspace,
+    its bytes)."""
+    shape, qs = _rows(q, "q", _HALF)
+    out_shape, os = _rows(out, "out", (q.dtype,))
+    if out_shape != shape:
+        raise ValueError(f"out {tuple(out_shape)} must have the shape of q {tuple(shape)}")
+    if cu is None or cu.numel() < 1:
         raise ValueError("cu: expected batch + 1 entries")
-    _vector(lse, "lse", (torch.float32,), q.shape[0] * q.shape[1])
+    cu_at, lse_at = _vector(cu, "cu", _INT), _vector(lse, "lse", (torch.float32,), shape[0] * shape[1])
     if workspace is None:
-        workspace = attention_workspace(q.shape[2], q.device)
+        workspace = attention_workspace(shape[2], q.device)
     _chk(workspace, "workspace")
-    return workspace, workspace.numel() * workspace.element_size(), q.shape[2] ** -0.5 if scale is None else scale
+    return shape, qs, os, cu_at, lse_at, workspace, workspace.numel() * workspace.element_size()
 
 
 def attention_packed(q, k, v, cu, out, *, scale=None, causal=True, lse=None, workspace=None):
     """Attention of packed sequences: rows cu[b] .. cu[b + 1] of q, out [T, Hq, d] and k, v [T, Hk, d] are sequence b.
     Query head h reads K/V head h // (Hq // Hk). scale defaults to d ** -0.5; lse (optional, fp32 [T, Hq]) gets the
     logarithm of each softmax denominator. Rows behind cu[-1] are left as they are."""
-    ws, ws_bytes, scale = _attention(q, out, cu, lse, workspace, scale)
-    _rows(k, "k", (q.dtype,)), _rows(v, "v", (q.dtype,))
-    tokens, hq, d = q.shape
-    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != d:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    (tokens, hq, d), qs, os, cu_at, lse_at, ws, ws_bytes = _attention(q, out, cu, lse, workspace)
+    shape, ks = _rows(k, "k", (q.dtype,))
+    v_shape, vs = _rows(v, "v", (q.dtype,))
+    if shape != v_shape or shape[0] != tokens or shape[2] != d:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v_shape)} do not fit q {tuple(q.shape)}")
     _here(q, k, v, cu, out, lse, ws)
-    lib().call("attention_packed", _stream(), _p(q), *_strides(q, 0, 1), _p(k), *_strides(k, 0, 1), _p(v), *_strides(v, 0, 1),
-               _p(out), *_strides(out, 0, 1), _code(q), _p(cu), cu.numel() - 1, tokens, hq, k.shape[1], d, scale, int(causal),
-               _p(lse), _p(ws), ws_bytes)
+    lib().call("attention_packed", _stream(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+               out.data_ptr(), os[0], os[1], _DT[q.dtype], cu_at, cu.numel() - 1, tokens, hq, shape[1], d,
+               d ** -0.5 if scale is None else scale, 1 if causal else 0, lse_at, ws.data_ptr(), ws_bytes)
     return out
 
 
@@ -434,16 +456,17 @@ def attention_paged(q, k_cache, v_cache, table, kv_len, cu, out, *, scale=None, 
     """Attention of new tokens over a paged cache that already holds them: rows cu[b] .. cu[b + 1] of q, out [T, Hq, d]
     are the newest of sequence b's kv_len[b] tokens, whose K and V stand in the pages table[b] of the caches
     [pages, page_size, Hk, d]. One row for each sequence is a decode step, more are a prompt's chunk, in any mixture."""
-    ws, ws_bytes, scale = _attention(q, out, cu, lse, workspace, scale)
-    pages, page_size, heads, d = _caches(k_cache, v_cache, (q.dtype,))
-    stride, cols = _table(table)
+    (tokens, hq, dq), qs, os, cu_at, lse_at, ws, ws_bytes = _attention(q, out, cu, lse, workspace)
+    (pages, page_size, heads, d), cs = _caches(k_cache, v_cache, (q.dtype,))
+    rows, cols, stride = _table(table)
     batch = cu.numel() - 1
-    _vector(kv_len, "kv_len", _INT, batch)
-    tokens, hq, dq = q.shape
-    if dq != d or table.shape[0] != batch:
+    if kv_len is None:
+        raise TypeError("kv_len is needed")
+    lens = _vector(kv_len, "kv_len", _INT, batch)
+    if dq != d or rows != batch:
         raise ValueError(f"q {tuple(q.shape)}, table {tuple(table.shape)} and cu do not fit caches {tuple(k_cache.shape)}")
     _here(q, k_cache, v_cache, table, kv_len, cu, out, lse, ws)
-    lib().call("attention_paged", _stream(), _p(q), *_strides(q, 0, 1), _p(k_cache), _p(v_cache), *_strides(k_cache, 0, 1, 2),
-               pages, page_size, _p(table), stride, cols, _p(kv_len), _p(out), *_strides(out, 0, 1), _code(q), _p(cu), batch,
-               tokens, hq, heads, d, scale, int(causal), _p(lse), _p(ws), ws_bytes)
+    lib().call("attention_paged", _stream(), q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+               pages, page_size, table.data_ptr(), stride, cols, lens, out.data_ptr(), os[0], os[1], _DT[q.dtype], cu_at, batch, tokens,
+               hq, heads, d, d ** -0.5 if scale is None else scale, 1 if causal else 0, lse_at, ws.data_ptr(), ws_bytes)
     return out
