@@ -45,7 +45,6 @@ constexpr uint32_t kSnap = 1;      // a border within so many tiles of a job's e
 constexpr uint32_t kMinShare = 3;  // least piece of work of a CTA
 constexpr uint32_t kMaxCtas = 148;
 constexpr float kLazy = 8.0f;      // log2 of the growth that a reference may lag behind
-constexpr uint32_t kTmemO = 256;   // TMEM columns: S0 0.., S1 128.., O 256..
 
 // CG CTAs (a pair of neighbouring SMs, or one) work on a tile of CG x 128 rows. A pair's tensor cores share the
 // operands: each CTA stages half of K (its keys) and half of V (its columns), which halves both the traffic from L2 and
@@ -55,20 +54,35 @@ struct Shape {
   static constexpr uint32_t kKeys = D == 256 && CG == 1 ? 64 : 128;    // keys of a tile
   static constexpr uint32_t kStageBytes = kKeys * D * 2 / CG;          // one CTA's share of a tile of K or V
   static constexpr uint32_t kQBytes = kRows * D * 2;
-  static constexpr uint32_t kStages = kStageBytes == 32768 ? 5 : 8;
+  static constexpr uint32_t kStages = kStageBytes != 32768 ? 8 : D == 256 ? 5 : 4;
   static constexpr uint32_t kKeyRows = kKeys / CG, kVChunks = D / 64 / CG;
   static constexpr uint32_t kParts = kKeys / 64;                       // P is handed on in parts of 64 keys
+  // TMEM, 512 columns: buffers of S (which P replaces) from 0, O at the end. With three buffers S(g + 2) is computed while
+  // P(g) waits for its product, and neither softmax group waits for S; two leave 128 + 2 x 128 columns at D = 256.
+  static constexpr uint32_t kBufs = D <= 128 ? 3 : 2, kAhead = kBufs - 1, kTmemO = 512 - D;
+  // Q of the next job is copied ahead where shared memory has room for a second one; where it has not, a job's products
+  // are finished before the next one's begin.
+  static constexpr uint32_t kQBufs = D <= 128 ? 2 : 1;
+  static constexpr bool kDrain = kQBufs == 1;
+  static constexpr uint32_t kSlots = kDrain ? 2 : 4;  // references and denominators in flight between the two groups
 };
 
-struct alignas(16) Shared {
-  unsigned long long kv_full[8], kv_empty[8], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], o_empty, v_dirty, v_clean, m_full[2][4], l_full[2][4];
+struct alignas(16) Basics {
   uint32_t tmem, abort;
   uint32_t start[4], end[4];  // (sequence, K/V head, row tile, key tile) of the piece's borders
-  float m[2][kRows];
-  float l[2][kRows];
 };
 template <int D, int CG>
-constexpr uint32_t kSmemBytes = Shape<D, CG>::kQBytes + Shape<D, CG>::kStages * Shape<D, CG>::kStageBytes + static_cast<uint32_t>(sizeof(Shared));
+struct alignas(16) Shared : Basics {
+  using Sh = Shape<D, CG>;
+  unsigned long long kv_full[Sh::kStages], kv_empty[Sh::kStages], q_full[Sh::kQBufs], q_empty[Sh::kQBufs];
+  unsigned long long s_full[Sh::kBufs], p_full[Sh::kBufs][Sh::kParts], pv_done[Sh::kBufs], o_empty, v_dirty, v_clean;
+  unsigned long long m_full[Sh::kSlots][4], l_full[Sh::kSlots][4];
+  float m[Sh::kSlots][kRows];
+  float l[Sh::kSlots][kRows];
+};
+template <int D, int CG>
+constexpr uint32_t kSmemBytes =
+    Shape<D, CG>::kQBufs * Shape<D, CG>::kQBytes + Shape<D, CG>::kStages * Shape<D, CG>::kStageBytes + static_cast<uint32_t>(sizeof(Shared<D, CG>));
 static_assert(kSmemBytes<256, 1> <= 232448 && kSmemBytes<256, 2> <= 232448 && kSmemBytes<128, 1> <= 232448 && kSmemBytes<128, 2> <= 232448 &&
                   kSmemBytes<64, 1> <= 232448,
               "shared memory of an SM");
@@ -206,7 +220,7 @@ __device__ __forceinline__ constexpr uint32_t instr_desc(uint32_t m, uint32_t n,
 }
 
 // A bounded wait; a thread whose wait runs out tells the others.
-__device__ __forceinline__ void wait(Shared& sh, unsigned long long* b, uint32_t parity) {
+__device__ __forceinline__ void wait(Basics& sh, unsigned long long* b, uint32_t parity) {
   const uint32_t bar = smem_addr(b);
   uint32_t done = 0;
   for (uint32_t spin = 0; spin < kStageSpinLimit && !done; ++spin) {
@@ -222,7 +236,7 @@ __device__ __forceinline__ void wait(Shared& sh, unsigned long long* b, uint32_t
   }
   if (!done && atomicExch(&sh.abort, 1u) == 0) atomicAdd(&g_attn_timeouts, 1u);
 }
-__device__ __forceinline__ bool aborted(Shared& sh) { return *reinterpret_cast<volatile uint32_t*>(&sh.abort) != 0; }
+__device__ __forceinline__ bool aborted(Basics& sh) { return *reinterpret_cast<volatile uint32_t*>(&sh.abort) != 0; }
 
 // ---- the line of work -----------------------------------------------------------------------------------------
 struct Seq {
@@ -376,7 +390,7 @@ struct Pieces {
   Seq s;
   // the present piece
   uint32_t t0, t1, n, keys;
-  __device__ __forceinline__ Pieces(const AttnCall& call, const Shared& sh, uint32_t tq_) : c(call), tq(tq_) {
+  __device__ __forceinline__ Pieces(const AttnCall& call, const Basics& sh, uint32_t tq_) : c(call), tq(tq_) {
     b = sh.start[0], h = sh.start[1], i = sh.start[2], t = sh.start[3];
     eb = sh.end[0], eh = sh.end[1], ei = sh.end[2], et = sh.end[3];
     if (b < c.batch) s = load_seq(c, b, tq);
@@ -462,10 +476,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Sh = Shape<D, CG>;
-  constexpr uint32_t KT = Sh::kKeys, ST = Sh::kStages, kChunks = D / 64;
+  constexpr uint32_t KT = Sh::kKeys, ST = Sh::kStages, kChunks = D / 64, NB = Sh::kBufs, NQ = Sh::kQBufs, NS = Sh::kSlots;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem_raw + Sh::kQBytes + ST * Sh::kStageBytes);
-  const uint32_t q_smem = smem_addr(smem_raw), kv_smem = q_smem + Sh::kQBytes;
+  auto& sh = *reinterpret_cast<Shared<D, CG>*>(smem_raw + NQ * Sh::kQBytes + ST * Sh::kStageBytes);
+  const uint32_t q_smem = smem_addr(smem_raw), kv_smem = q_smem + NQ * Sh::kQBytes;
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const uint32_t rank = CG == 2 ? blockIdx.x & 1u : 0u, unit = blockIdx.x / CG, units = gridDim.x / CG;
   const uint32_t tq_cta = kRows / c.group, tq = CG * tq_cta;  // tokens of a CTA's rows, of a row tile
@@ -474,17 +488,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // a pair's products need both CTAs' operands: the leader's barriers count the other's arrivals too
     const uint32_t both = rank == 0 ? CG : 1;
     for (uint32_t i = 0; i < ST; ++i) bar_init(&sh.kv_full[i], both), bar_init(&sh.kv_empty[i], 1);
-    bar_init(&sh.q_full, both);
-    bar_init(&sh.q_empty, 1);
+    for (uint32_t i = 0; i < NQ; ++i) bar_init(&sh.q_full[i], both), bar_init(&sh.q_empty[i], 1);
     bar_init(&sh.v_dirty, 1);
     bar_init(&sh.v_clean, 1);
     bar_init(&sh.o_empty, 4 * CG);
-    for (int i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < NB; ++i) {
       bar_init(&sh.s_full[i], 1);
-      for (int w = 0; w < 2; ++w) bar_init(&sh.p_full[i][w], 4 * CG);
+      for (uint32_t w = 0; w < Sh::kParts; ++w) bar_init(&sh.p_full[i][w], 4 * CG);
       bar_init(&sh.pv_done[i], 1);
-      for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1), bar_init(&sh.l_full[i][w], 1);
     }
+    for (uint32_t i = 0; i < NS; ++i)
+      for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1), bar_init(&sh.l_full[i][w], 1);
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -518,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Pieces<KT> pc(c, sh, tq);
     if (warp == 8) {
       // ---- copies -------------------------------------------------------------------------------------------------
-      uint32_t g = 0, fill = 0, job = 0;
+      uint32_t fill = 0, job = 0;
       uint32_t issued = 0;  // stages that have had a load
       const uint32_t q_bytes = tq_cta * c.group * 128u * kChunks;
       // One operand's tile: up to `kMost` key rows from key0 on, kCh chunks of 64 columns from `col` on, laid out
@@ -553,23 +567,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
       };
-      // order of use in a job: K(0), K(1), V(0), K(2), V(1), ...
-      uint32_t pb = 0, ph = 0, pt = 0, pkeys = 0, prow = 0;
+      // The order of use, which is also the order of the stages: K(g), V(g - kAhead), ..., what is left of V at the end
+      // (and, where Q has one buffer, at the end of each job).
+      struct Tile {
+        uint32_t row0, b, h, t, keys;
+      } last[Sh::kAhead];
+      uint32_t left = 0;  // tiles whose V is still to come
       const uint32_t vcol = uniform(rank * (D / CG));
-      auto load_v = [&](uint32_t slot) { load_kv(Int<KT>{}, Int<Sh::kVChunks>{}, &vmap, prow, pb, ph, pt * KT, pkeys, vcol, slot); };
+      auto load_v = [&] {
+        const Tile& v = left == 1 ? last[0] : last[Sh::kAhead - 1];
+        load_kv(Int<KT>{}, Int<Sh::kVChunks>{}, &vmap, v.row0, v.b, v.h, v.t * KT, v.keys, vcol, fill++);
+        --left;
+      };
       for (; pc.next() && !aborted(sh); pc.advance()) {
-        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
-          // the stages are used in this order, whichever is asked for first: K(g) ahead of V(g - 1), but behind it at
-          // the start of a job, whose Q can only be copied once the last job's products with Q are done
-          const bool k_ahead = t > pc.t0 && g > 0;
-          const uint32_t kslot = fill + (k_ahead || g == 0 ? 0u : 1u), vslot = fill + (k_ahead ? 1u : 0u);
-          fill += g > 0 ? 2u : 1u;
-          if (g > 0) load_v(vslot);
+        for (uint32_t t = pc.t0; t < pc.t1; ++t) {
           if (t == pc.t0) {
-            if (job > 0) wait(sh, &sh.q_empty, (job - 1) & 1u);
+            if constexpr (Sh::kDrain)
+              while (left) load_v();
+            const uint32_t qb = uniform(job % NQ);
+            if (job >= NQ) wait(sh, &sh.q_empty[qb], (job / NQ - 1) & 1u);
             if (aborted(sh)) break;
-            const uint32_t bar = uniform(smem_addr(&sh.q_full)), head = uniform(pc.h * c.group), tok = uniform(pc.s.row0 + pc.i * tq + rank * tq_cta);
-            const uint32_t to = uniform(q_smem);
+            const uint32_t bar = uniform(smem_addr(&sh.q_full[qb])), head = uniform(pc.h * c.group), tok = uniform(pc.s.row0 + pc.i * tq + rank * tq_cta);
+            const uint32_t to = uniform(q_smem + qb * Sh::kQBytes);
             if (elect()) {
               stage_expect(bar, q_bytes);
 #pragma unroll
@@ -579,15 +598,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             ++job;
           }
-          load_kv(Int<Sh::kKeyRows>{}, Int<kChunks>{}, &kmap, pc.s.row0, pc.b, pc.h, t * KT + rank * Sh::kKeyRows, pc.keys, 0, kslot);
-          prow = pc.s.row0, pb = pc.b, ph = pc.h, pt = t, pkeys = pc.keys;
+          load_kv(Int<Sh::kKeyRows>{}, Int<kChunks>{}, &kmap, pc.s.row0, pc.b, pc.h, t * KT + rank * Sh::kKeyRows, pc.keys, 0, fill++);
+          if (left == Sh::kAhead) load_v();
+#pragma unroll
+          for (uint32_t i = Sh::kAhead - 1; i > 0; --i) last[i] = last[i - 1];
+          last[0] = Tile{pc.s.row0, pc.b, pc.h, t, pc.keys};
+          ++left;
         }
       }
-      if (g > 0 && !aborted(sh)) load_v(fill++);
+      while (left && !aborted(sh)) load_v();
       // every stage's last use is over before the CTA may leave: no arrival of the other CTA's products is under way
       if (!aborted(sh)) {
         for (uint32_t i = fill > ST ? fill - ST : 0u; i < fill; ++i) wait(sh, &sh.kv_empty[i % ST], (i / ST) & 1u);
-        if (job) wait(sh, &sh.q_empty, (job - 1) & 1u);
+        for (uint32_t i = job > NQ ? job - NQ : 0u; i < job; ++i) wait(sh, &sh.q_empty[i % NQ], (i / NQ) & 1u);
       }
       if (aborted(sh)) {
         // no copy may land in shared memory that another CTA owns by then: one more bounded wait for each
@@ -596,9 +619,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             stage_wait(smem_addr(&sh.kv_full[st]), 0);
             stage_wait(smem_addr(&sh.kv_full[st]), 1);
           }
-        if (job) {
-          stage_wait(smem_addr(&sh.q_full), 0);
-          stage_wait(smem_addr(&sh.q_full), 1);
+        for (uint32_t i = 0; i < min(job, NQ); ++i) {
+          stage_wait(smem_addr(&sh.q_full[i]), 0);
+          stage_wait(smem_addr(&sh.q_full[i]), 1);
         }
       }
     } else if (warp == 9 && rank == 0) {
@@ -606,28 +629,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc_s = instr_desc<T>(CG * kRows, KT, false), idesc_o = instr_desc<T>(CG * kRows, D, true);
       const uint32_t qs = uniform(q_smem), kvs = uniform(kv_smem), tm = uniform(tmem);
       uint32_t g = 0, job = 0, tails = 0, st = 0, ph = 0;  // the stages are used in the order in which they are filled
-      uint32_t first = 0, tail = 0, prev_job = 0;          // of tile g - 1
+      uint32_t sb = 0, pb = 0, pph = 0;                    // buffer of the next S, of the next P, and its phase
+      uint32_t left = 0;                                   // tiles whose P V is still to come
+      struct Tile {
+        uint32_t first, tail, job;
+      } last[Sh::kAhead];
       auto next_stage = [&] {
         if (++st == ST) st = 0, ph ^= 1u;
       };
-      auto pv = [&](uint32_t gt) {
-        const uint32_t buf = uniform(gt & 1u);
+      auto pv = [&] {
+        const Tile& v = left == 1 ? last[0] : last[Sh::kAhead - 1];
+        const uint32_t buf = uniform(pb), acc = uniform(v.first) ^ 1u;
         const uint64_t d = smem_desc(kvs + uniform(st) * Sh::kStageBytes, KT * 128u);
-        const uint32_t acc = uniform(first) ^ 1u;
         wait(sh, &sh.kv_full[st], ph);
-        if (tail) {
+        if (v.tail) {
           if (lane == 0) bar_arrive(&sh.v_dirty);
           wait(sh, &sh.v_clean, tails++ & 1u);
         }
-        if (first && prev_job > 0) wait(sh, &sh.o_empty, (prev_job - 1) & 1u);
+        if (v.first && v.job > 0) wait(sh, &sh.o_empty, (v.job - 1) & 1u);
 #pragma unroll
         for (uint32_t part = 0; part < Sh::kParts; ++part) {
-          wait(sh, &sh.p_full[buf][part], (gt >> 1) & 1u);
+          wait(sh, &sh.p_full[buf][part], pph);
           tc_after();
           if (elect()) {
 #pragma unroll
             for (uint32_t k = part * 4; k < part * 4 + 4; ++k)
-              mma_ts<CG>(tm + kTmemO, tm + buf * 128u + k * 8u, d + k * (2048u >> 4), idesc_o, k == 0 ? acc : 1u);
+              mma_ts<CG>(tm + Sh::kTmemO, tm + buf * KT + k * 8u, d + k * (2048u >> 4), idesc_o, k == 0 ? acc : 1u);
             if (part + 1 == Sh::kParts) {
               tc_commit<CG>(&sh.kv_empty[st]);
               tc_commit<CG>(&sh.pv_done[buf]);
@@ -636,42 +663,51 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         next_stage();
+        if (++pb == NB) pb = 0, pph ^= 1u;
+        --left;
       };
       for (; pc.next() && !aborted(sh); pc.advance()) {
         const uint32_t t0 = uniform(pc.t0), t1 = uniform(pc.t1);
         for (uint32_t t = t0; t < t1; ++t, ++g) {
-          if (t == t0 && g > 0) pv(g - 1);
-          const uint32_t buf = uniform(g & 1u);
-          const uint64_t qd = smem_desc(qs, 16), d = smem_desc(kvs + uniform(st) * Sh::kStageBytes, 16);
-          if (t == t0) wait(sh, &sh.q_full, job & 1u);
+          const uint32_t qb = uniform(job % NQ), buf = uniform(sb);
+          if (t == t0) {
+            if constexpr (Sh::kDrain)
+              while (left) pv();
+            wait(sh, &sh.q_full[qb], (job / NQ) & 1u);
+          }
+          const uint64_t qd = smem_desc(qs + qb * Sh::kQBytes, 16), d = smem_desc(kvs + uniform(st) * Sh::kStageBytes, 16);
           wait(sh, &sh.kv_full[st], ph);
           if (elect()) {
 #pragma unroll
             for (uint32_t k = 0; k < D / 16; ++k)
-              mma_ss<CG>(tm + buf * 128u, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u,
+              mma_ss<CG>(tm + buf * KT, qd + ((k >> 2) * kRows * 128u + (k & 3u) * 32u) / 16u,
                          d + ((k >> 2) * Sh::kKeyRows * 128u + (k & 3u) * 32u) / 16u, idesc_s, k > 0);
             tc_commit<CG>(&sh.kv_empty[st]);
             tc_commit<CG>(&sh.s_full[buf]);
-            if (t + 1 == t1) tc_commit<CG>(&sh.q_empty);
+            if (t + 1 == t1) tc_commit<CG>(&sh.q_empty[qb]);
           }
           __syncwarp();
           next_stage();
-          if (t > t0) pv(g - 1);
-          first = t == t0;
-          tail = pc.keys - t * KT < KT;
-          prev_job = job;
+          if (++sb == NB) sb = 0;
+          if (left == Sh::kAhead) pv();
+#pragma unroll
+          for (uint32_t i = Sh::kAhead - 1; i > 0; --i) last[i] = last[i - 1];
+          last[0] = Tile{t == t0, pc.keys - t * KT < KT, job};
+          ++left;
         }
         if (t1 > t0) ++job;
       }
-      if (g > 0 && !aborted(sh)) pv(g - 1);
+      while (left && !aborted(sh)) pv();
     } else if (warp == 10) {
       // ---- V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: they are
       // cleared. And a pair's second CTA tells the leader what has landed.
-      uint32_t g = 0, st = 0, ph = 0, jobs = 0, tails = 0, valid = KT;
+      uint32_t st = 0, ph = 0, jobs = 0, tails = 0, left = 0;
+      uint32_t last[Sh::kAhead];  // keys of the tiles whose V is still to come
       auto next_stage = [&] {
         if (++st == ST) st = 0, ph ^= 1u;
       };
       auto v_stage = [&] {
+        const uint32_t valid = left == 1 ? last[0] : last[Sh::kAhead - 1];
         // the second CTA's stage waits for its word, the leader's only where the multiplying thread asked for it
         if (rank) wait(sh, &sh.kv_full[st], ph);
         else if (valid < KT) wait(sh, &sh.v_dirty, tails++ & 1u);
@@ -693,25 +729,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && rank) bar_arrive_leader(&sh.kv_full[st]);
         __syncwarp();
         next_stage();
+        --left;
       };
       for (; pc.next() && !aborted(sh); pc.advance()) {
-        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
-          if (t == pc.t0 && g > 0) v_stage();
-          if (rank) {
-            if (t == pc.t0) {
-              wait(sh, &sh.q_full, jobs++ & 1u);
-              if (lane == 0) bar_arrive_leader(&sh.q_full);
+        for (uint32_t t = pc.t0; t < pc.t1; ++t) {
+          if (t == pc.t0) {
+            if constexpr (Sh::kDrain)
+              while (left) v_stage();
+            if (rank) {
+              wait(sh, &sh.q_full[jobs % NQ], (jobs / NQ) & 1u);
+              if (lane == 0) bar_arrive_leader(&sh.q_full[jobs % NQ]);
+              ++jobs;
             }
+          }
+          if (rank) {
             wait(sh, &sh.kv_full[st], ph);
             if (lane == 0) bar_arrive_leader(&sh.kv_full[st]);
             __syncwarp();
           }
           next_stage();
-          if (t > pc.t0) v_stage();
-          valid = min(KT, pc.keys - t * KT);
+          if (left == Sh::kAhead) v_stage();
+#pragma unroll
+          for (uint32_t i = Sh::kAhead - 1; i > 0; --i) last[i] = last[i - 1];
+          last[0] = min(KT, pc.keys - t * KT);
+          ++left;
         }
       }
-      if (g > 0 && !aborted(sh)) v_stage();
+      while (left && !aborted(sh)) v_stage();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -736,15 +780,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t all_see = c.causal ? static_cast<uint32_t>(max(0, pc.s.off + static_cast<int>(tok0) + 1)) : pc.keys;
       float m = -INFINITY, l = 0.0f;  // the reference that l is relative to
       float before = -INFINITY;       // the one of the tile before
-      for (uint32_t t = pc.t0; t < pc.t1; ++t, ++g) {
-        const uint32_t buf = g & 1u;
-        if (buf != wg) continue;
-        wait(sh, &sh.s_full[buf], (g >> 1) & 1u);
+      const uint32_t g0 = g;
+      g += pc.t1 - pc.t0;
+      for (uint32_t t = pc.t0 + ((g0 ^ wg) & 1u); t < pc.t1; t += 2) {
+        const uint32_t g = g0 + (t - pc.t0);
+        const uint32_t buf = g % NB, slot = g % NS;
+        wait(sh, &sh.s_full[buf], (g / NB) & 1u);
         tc_after();
         if (busy) {
           float s[KT / 32][32];
 #pragma unroll
-          for (uint32_t x = 0; x < KT / 32; ++x) tc_ld32(tmem + lane_base + buf * 128u + x * 32u, s[x]);
+          for (uint32_t x = 0; x < KT / 32; ++x) tc_ld32(tmem + lane_base + buf * KT + x * 32u, s[x]);
+          float ref = -INFINITY;  // the other group's, of the tile before
+          if (t > pc.t0) {
+            wait(sh, &sh.m_full[(g - 1) % NS][quad], ((g - 1) / NS) & 1u);
+            ref = sh.m[(g - 1) % NS][row];
+          }
+          before = ref;
           tc_wait_ld(s);
           const uint32_t key0 = t * KT;
           if (key0 + KT > min(all_see, pc.keys)) {
@@ -757,39 +809,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(keep & (1u << y))) s[x][y] = -INFINITY;
             }
           }
-          float mx = -INFINITY;
+          float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains
 #pragma unroll
-          for (uint32_t x = 0; x < KT; x += 2) mx = max3f(mx, s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
+          for (uint32_t x = 0; x < KT; x += 2) part[x / 2 % 4] = max3f(part[x / 2 % 4], s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
+          float mx = fmaxf(max3f(part[0], part[1], part[2]), part[3]);
           if (row >= rows) mx = -INFINITY;  // no query row: what stands there has no say
-          float ref = -INFINITY;
-          if (t > pc.t0) {
-            wait(sh, &sh.m_full[buf ^ 1u][quad], ((g - 1) >> 1) & 1u);
-            ref = sh.m[buf ^ 1u][row];
-          }
-          before = ref;
           // the reference follows where it has fallen too far behind
           const float grown = __fmul_rn(mx - ref, c.scale_log2);
           const bool follow = grown > kLazy;  // also from -inf; false for -inf against -inf (NaN)
           const float next_ref = follow ? mx : ref;
           if (__any_sync(kFullMask, follow && ref != -INFINITY)) {
-            wait(sh, &sh.pv_done[buf ^ 1u], ((g - 1) >> 1) & 1u);
+            wait(sh, &sh.pv_done[(g - 1) % NB], ((g - 1) / NB) & 1u);
             tc_after();
             const float f = follow && ref != -INFINITY ? ex2_approx(-grown) : 1.0f;
 #pragma unroll 1
             for (uint32_t x = 0; x < D / 32; ++x) {
               float o[32];
-              tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
+              tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u, o);
               tc_wait_ld(o);
               uint32_t r[32];
 #pragma unroll
               for (int y = 0; y < 32; ++y) r[y] = __float_as_uint(__fmul_rn(o[y], f));
-              tc_st32(tmem + lane_base + kTmemO + x * 32u, r);
+              tc_st32(tmem + lane_base + Sh::kTmemO + x * 32u, r);
             }
             tc_wait_st();
           }
-          sh.m[buf][row] = next_ref;
+          sh.m[slot][row] = next_ref;
           __syncwarp();
-          if (lane == 0) bar_arrive(&sh.m_full[buf][quad]);
+          if (lane == 0) bar_arrive(&sh.m_full[slot][quad]);
           // p = 2^(c s - c ref); a row that has seen nothing yet has s = -inf everywhere, and 0 does for its reference
           const float mc = next_ref == -INFINITY ? 0.0f : __fmul_rn(next_ref, c.scale_log2);
           const float2 c2 = make_float2(c.scale_log2, c.scale_log2), m2 = make_float2(-mc, -mc);
@@ -806,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum = __fadd2_rn(sum, v);
               r[y] = pack2<T>(v.x, v.y);
             }
-            tc_st32(tmem + lane_base + buf * 128u + x * 32u, r);
+            tc_st32(tmem + lane_base + buf * KT + x * 32u, r);
             if (x + 1 < Sh::kParts) {  // the first part goes to the tensor cores while the second is computed
               tc_wait_st();
               tc_before();
@@ -822,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_wait_st();
         } else {
           if (lane == 0) {
-            bar_arrive(&sh.m_full[buf][quad]);
+            bar_arrive(&sh.m_full[slot][quad]);
             for (uint32_t x = 0; x + 1 < Sh::kParts; ++x) tell_leader(&sh.p_full[buf][x]);
           }
         }
@@ -832,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const bool any = pc.t1 > pc.t0, whole = pc.t0 == 0 && pc.t1 == pc.n;
       const bool both_groups = pc.t1 - pc.t0 >= 2;
-      const uint32_t shared = shares & 1u, share_phase = (shares >> 1) & 1u;
+      const uint32_t shared = shares % NS, share_phase = (shares / NS) & 1u;
       if (both_groups) ++shares;
       // The group of the last tile writes the outputs, while the other one, having left its denominator behind, goes on
       // to the next job's first tile.
@@ -854,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           else if (before != -INFINITY) total = __fmaf_rn(other, ex2_approx(__fmul_rn(before - ref, c.scale_log2)), total);
         }
         if (any) {
-          wait(sh, &sh.pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u);
+          wait(sh, &sh.pv_done[(g - 1) % NB], ((g - 1) / NB) & 1u);
           tc_after();
         }
         const bool mine = row < rows && !aborted(sh);
@@ -871,8 +918,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (uint32_t x = 0; x < D / 32; x += 2) {
             float o[2][32];
-            tc_ld32(tmem + lane_base + kTmemO + x * 32u, o[0]);
-            tc_ld32(tmem + lane_base + kTmemO + x * 32u + 32u, o[1]);
+            tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u, o[0]);
+            tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u + 32u, o[1]);
             tc_wait_ld(o);
 #pragma unroll
             for (uint32_t z = 0; z < 2; ++z) {
@@ -904,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (uint32_t x = 0; x < D / 32; ++x) {
             float o[32];
-            tc_ld32(tmem + lane_base + kTmemO + x * 32u, o);
+            tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u, o);
             tc_wait_ld(o);
             // [column / 4][row] quads, so that a warp's rows lie side by side
             if (mine) {
