@@ -2,7 +2,8 @@
 
     python -m halo_flash_b200.build [--force] [--verbose]
 
-Objects go to halo_flash_b200/csrc/build/, the library to halo_flash_b200/libhalo_b200.so.
+Objects go to halo_flash_b200/csrc/build/, the library to halo_flash_b200/libhalo_b200.so, and beside it the
+extension module through which ops.py makes its attention calls (csrc/bind.cpp, host code only).
 A source is recompiled when it or any header is newer than its object.
 """
 from __future__ import annotations
@@ -12,7 +13,9 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib.util import find_spec
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -20,6 +23,7 @@ CSRC = PKG / "csrc"
 OBJ = CSRC / "build"
 LIB = PKG / "libhalo_b200.so"
 INCLUDE = PKG.parent / "include"
+BIND = PKG / ("_bind" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 SOURCES = ["norm.cu", "norm_odd.cu", "rope.cu", "elementwise.cu", "embed.cu", "quant.cu", "hc.cu", "conv.cu", "paged.cu", "attention.cu", "api.cu", "launch.cu", "static_scratch.cu"]
 
@@ -44,6 +48,21 @@ def _stale(target: Path, deps: list[Path]) -> bool:
         return True
     t = target.stat().st_mtime
     return any(d.stat().st_mtime > t for d in deps)
+
+
+def _build_bind(nvcc: str, force: bool) -> None:
+    src = CSRC / "bind.cpp"
+    if not force and not _stale(BIND, [src, INCLUDE / "halo_b200.h", Path(__file__)]):
+        return
+    torch = Path(find_spec("torch").submodule_search_locations[0])
+    cuda = Path(nvcc).resolve().parents[1]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(INCLUDE), "-I", sysconfig.get_paths()["include"],
+           "-isystem", str(torch / "include"), "-isystem", str(torch / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
+           str(src), "-o", str(BIND), "-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-L", str(PKG), "-lhalo_b200", "-Wl,-rpath,$ORIGIN"]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"g++ failed on bind.cpp:\n{p.stdout}\n{p.stderr}")
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -78,6 +97,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         p = subprocess.run(cmd, capture_output=True, text=True)
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n{p.stdout}\n{p.stderr}")
+    _build_bind(nvcc, force)
     return LIB
 
 

@@ -323,59 +323,23 @@ def moe_combine(yp, pos, mw, out, *, sx=None, sg=None):
 
 
 # ---- paged K/V cache and attention ----------------------------------------------------------------
-# A decode step calls these for every layer with a few rows, so what they do on the host is kept short.
-_INT = (torch.int32, torch.uint32)
-_I64 = (torch.int64,)
-_HALF = (torch.float16, torch.bfloat16)
-_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+# A decode step makes these calls for every layer with a few rows, so the tensors are checked and unpacked by an
+# extension module (csrc/bind.cpp). Every tensor has to be on the current device; rows and caches may be views of any
+# strides whose last axis is contiguous.
+_bound = None
 
 
-def _here(*tensors):
-    """The kernels run on the current device's current stream: every tensor must live there."""
-    device = _device()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{device}")
-    return device
-
-
-def _rows(t, name, dtypes, rank=3):
-    """(shape, strides) of a CUDA tensor of `rank` axes whose last one is contiguous; the other strides are free."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name}: expected a CUDA tensor (halo_flash_b200 has no CPU path)")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name}: dtype {t.dtype} not in {dtypes}")
-    shape, strides = t.shape, t.stride()
-    if len(shape) != rank:
-        raise ValueError(f"{name}: expected {rank} axes, got shape {tuple(shape)}")
-    if strides[-1] != 1 and shape[-1] > 1:
-        raise ValueError(f"{name}: the last axis must be contiguous")
-    return shape, strides
-
-
-def _caches(k_cache, v_cache, dtypes):
-    shape, strides = _rows(k_cache, "k_cache", dtypes, 4)
-    v_shape, v_strides = _rows(v_cache, "v_cache", (k_cache.dtype,), 4)
-    if shape != v_shape or (strides != v_strides and any(a != b and n > 1 for a, b, n in zip(strides, v_strides, shape))):
-        raise ValueError("k_cache and v_cache must have the same shape and strides")
-    return shape, strides
-
-
-def _table(table):
-    (rows, cols), (stride, _) = _rows(table, "table", _INT, 2)
-    if rows > 1 and stride < cols:
-        raise ValueError("table: rows overlap")
-    return rows, cols, stride
-
-
-def _vector(t, name, dtypes, n=None):
-    """The address of a contiguous CUDA tensor of n entries, None for None."""
-    if t is None:
-        return None
-    _chk(t, name, dtypes)
-    if n is not None and t.numel() != n:
-        raise ValueError(f"{name}: expected {n} entries, got {t.numel()}")
-    return t.data_ptr()
+def _bind():
+    global _bound
+    if _bound is None:
+        lib()  # says so when the library itself is not built
+        try:
+            from . import _bind as module
+        except ImportError as e:
+            raise FileNotFoundError("halo_flash_b200/_bind is missing or does not load: build it with "
+                                    "`python -m halo_flash_b200.build`") from e
+        _bound = module
+    return _bound
 
 
 def paged_plan(table, past, fresh, free_pages, page_size, slot, *, pos=None, cu=None, kv_len=None, status=None):
@@ -384,34 +348,14 @@ def paged_plan(table, past, fresh, free_pages, page_size, slot, *, pos=None, cu=
     token's page * page_size + offset (-1: refused, or behind the last new token), pos its position, cu [B + 1] the
     prefix sum of fresh, kv_len past + fresh, status [pages taken, requests refused, new tokens]. A request that the
     table row or the free list cannot hold is refused: no pages, slots -1, kv_len = past."""
-    if slot is None or past is None or fresh is None or free_pages is None:
-        raise TypeError("past, fresh, free_pages and slot are needed")
-    batch, cols, stride = _table(table)
-    slots = _vector(slot, "slot", _I64)
-    tokens = slot.numel()
-    args = (table.data_ptr(), stride, cols, _vector(past, "past", _INT, batch), _vector(fresh, "fresh", _INT, batch),
-            _vector(free_pages, "free_pages", _INT), free_pages.numel(), page_size, slots, _vector(pos, "pos", _INT, tokens),
-            _vector(cu, "cu", _INT, batch + 1), _vector(kv_len, "kv_len", _INT, batch), _vector(status, "status", _INT, 3), batch, tokens)
-    _here(table, past, fresh, free_pages, slot, pos, cu, kv_len, status)
-    lib().call("paged_plan", _stream(), *args)
+    (_bound or _bind()).paged_plan(table, past, fresh, free_pages, page_size, slot, pos, cu, kv_len, status)
     return slot
 
 
 def paged_store(k, v, k_cache, v_cache, slot):
     """Rows k, v [T, heads, d] to the rows of the caches [pages, page_size, heads, d] that slot (int64 [T]) names;
-    slots outside the cache are skipped, and no two of a call may be equal. The caches may be views of any strides."""
-    (pages, page_size, heads, d), cs = _caches(k_cache, v_cache, _ACT)
-    shape, ks = _rows(k, "k", _ACT)
-    v_shape, vs = _rows(v, "v", (k.dtype,))
-    tokens = shape[0]
-    if shape != v_shape or shape[1] != heads or shape[2] != d:
-        raise ValueError(f"k {tuple(shape)} and v {tuple(v_shape)} do not fit caches of {heads} heads of {d}")
-    if slot is None:
-        raise TypeError("slot is needed")
-    slots = _vector(slot, "slot", _I64, tokens)
-    _here(k, v, k_cache, v_cache, slot)
-    lib().call("paged_store", _stream(), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _DT[k.dtype], k_cache.data_ptr(),
-               v_cache.data_ptr(), _DT[k_cache.dtype], cs[0], cs[1], cs[2], pages, page_size, slots, heads, d, tokens)
+    slots outside the cache are skipped, and no two of a call may be equal."""
+    (_bound or _bind()).paged_store(k, v, k_cache, v_cache, slot)
 
 
 def attention_workspace(d, device=None):
@@ -420,35 +364,11 @@ def attention_workspace(d, device=None):
     return torch.empty(lib().cdll.halo_b200_attention_workspace(d), dtype=torch.uint8, device=device or "cuda")
 
 
-def _attention(q, out, cu, lse, workspace):
-    """What both forms check and pass on: (q's shape and strides, out's strides, addresses of cu, lse and the workspace,
-    its bytes)."""
-    shape, qs = _rows(q, "q", _HALF)
-    out_shape, os = _rows(out, "out", (q.dtype,))
-    if out_shape != shape:
-        raise ValueError(f"out {tuple(out_shape)} must have the shape of q {tuple(shape)}")
-    if cu is None or cu.numel() < 1:
-        raise ValueError("cu: expected batch + 1 entries")
-    cu_at, lse_at = _vector(cu, "cu", _INT), _vector(lse, "lse", (torch.float32,), shape[0] * shape[1])
-    if workspace is None:
-        workspace = attention_workspace(shape[2], q.device)
-    _chk(workspace, "workspace")
-    return shape, qs, os, cu_at, lse_at, workspace, workspace.numel() * workspace.element_size()
-
-
 def attention_packed(q, k, v, cu, out, *, scale=None, causal=True, lse=None, workspace=None):
     """Attention of packed sequences: rows cu[b] .. cu[b + 1] of q, out [T, Hq, d] and k, v [T, Hk, d] are sequence b.
     Query head h reads K/V head h // (Hq // Hk). scale defaults to d ** -0.5; lse (optional, fp32 [T, Hq]) gets the
     logarithm of each softmax denominator. Rows behind cu[-1] are left as they are."""
-    (tokens, hq, d), qs, os, cu_at, lse_at, ws, ws_bytes = _attention(q, out, cu, lse, workspace)
-    shape, ks = _rows(k, "k", (q.dtype,))
-    v_shape, vs = _rows(v, "v", (q.dtype,))
-    if shape != v_shape or shape[0] != tokens or shape[2] != d:
-        raise ValueError(f"k {tuple(shape)} and v {tuple(v_shape)} do not fit q {tuple(q.shape)}")
-    _here(q, k, v, cu, out, lse, ws)
-    lib().call("attention_packed", _stream(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-               out.data_ptr(), os[0], os[1], _DT[q.dtype], cu_at, cu.numel() - 1, tokens, hq, shape[1], d,
-               d ** -0.5 if scale is None else scale, 1 if causal else 0, lse_at, ws.data_ptr(), ws_bytes)
+    (_bound or _bind()).attention_packed(q, k, v, cu, out, scale, causal, lse, workspace)
     return out
 
 
@@ -456,17 +376,5 @@ def attention_paged(q, k_cache, v_cache, table, kv_len, cu, out, *, scale=None, 
     """Attention of new tokens over a paged cache that already holds them: rows cu[b] .. cu[b + 1] of q, out [T, Hq, d]
     are the newest of sequence b's kv_len[b] tokens, whose K and V stand in the pages table[b] of the caches
     [pages, page_size, Hk, d]. One row for each sequence is a decode step, more are a prompt's chunk, in any mixture."""
-    (tokens, hq, dq), qs, os, cu_at, lse_at, ws, ws_bytes = _attention(q, out, cu, lse, workspace)
-    (pages, page_size, heads, d), cs = _caches(k_cache, v_cache, (q.dtype,))
-    rows, cols, stride = _table(table)
-    batch = cu.numel() - 1
-    if kv_len is None:
-        raise TypeError("kv_len is needed")
-    lens = _vector(kv_len, "kv_len", _INT, batch)
-    if dq != d or rows != batch:
-        raise ValueError(f"q {tuple(q.shape)}, table {tuple(table.shape)} and cu do not fit caches {tuple(k_cache.shape)}")
-    _here(q, k_cache, v_cache, table, kv_len, cu, out, lse, ws)
-    lib().call("attention_paged", _stream(), q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
-               pages, page_size, table.data_ptr(), stride, cols, lens, out.data_ptr(), os[0], os[1], _DT[q.dtype], cu_at, batch, tokens,
-               hq, heads, d, d ** -0.5 if scale is None else scale, 1 if causal else 0, lse_at, ws.data_ptr(), ws_bytes)
+    (_bound or _bind()).attention_paged(q, k_cache, v_cache, table, kv_len, cu, out, scale, causal, lse, workspace)
     return out

@@ -72,3 +72,17 @@ def test_empty_calls_are_no_ops():
     lib.call("attention_paged", None, *_paged(tokens=0))
     lib.call("paged_store", None, A, 1, 1, A, 1, 1, 2, A, A, 2, 1, 1, 1, 4, 64, A, 2, 64, 0)
     lib.call("paged_plan", None, None, 0, 0, None, None, None, 0, 64, None, None, None, None, None, 0, 0)
+
+
+def test_ops_refuse_what_is_no_cuda_tensor():
+    """The extension module's own checks, as far as they go without a device."""
+    import torch
+    from halo_flash_b200 import ops
+    t = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    c = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
+    i = torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: ops.attention_packed(t, t, t, i, t), lambda: ops.attention_packed(None, t, t, i, t),
+                 lambda: ops.attention_paged(t, c, c, i[None], i, i, t), lambda: ops.paged_store(t, t, c, c, i.long()),
+                 lambda: ops.paged_plan(i[None], i, i, i, 16, i.long()), lambda: ops.paged_plan([1], i, i, i, 16, i.long())):
+        with pytest.raises(TypeError, match="CUDA tensor"):
+            call()

@@ -272,3 +272,37 @@ def test_no_wait_ran_out():
     import ctypes as C
     n, err = C.c_uint(99), C.create_string_buffer(256)
     assert lib().cdll.halo_b200_stage_timeouts(C.byref(n), err, len(err)) == 0 and n.value == 0
+
+
+def test_tensor_refusals():
+    """What ops checks of the tensors; each call is refused on the host, before anything is launched."""
+    q, k, out = (torch.zeros(6, h, 64, dtype=BF16, device=DEV) for h in (4, 2, 4))
+    cu, lens, table = _i32([0, 6]), _i32([6]), _i32([[0, 1]])
+    kc = torch.zeros(3, 16, 2, 64, dtype=BF16, device=DEV)
+    slot = torch.zeros(6, dtype=torch.int64, device=DEV)
+    packed = lambda **kw: ops.attention_packed(**{**dict(q=q, k=k, v=k, cu=cu, out=out), **kw})  # noqa: E731
+    paged = lambda **kw: ops.attention_paged(**{**dict(q=q, k_cache=kc, v_cache=kc, table=table, kv_len=lens, cu=cu, out=out), **kw})  # noqa: E731
+    store = lambda **kw: ops.paged_store(**{**dict(k=k, v=k, k_cache=kc, v_cache=kc, slot=slot), **kw})  # noqa: E731
+    plan = lambda **kw: ops.paged_plan(**{**dict(table=table, past=lens, fresh=lens, free_pages=lens, page_size=16, slot=slot), **kw})  # noqa: E731
+    for error, word, call in (
+            (TypeError, "dtype", lambda: packed(q=q.float())), (TypeError, "out's|q's", lambda: packed(out=out.half())),
+            (TypeError, "q's", lambda: packed(k=k.half())), (ValueError, "axes", lambda: packed(q=q[0])), (ValueError, "shape of q", lambda: packed(out=out[:5])),
+            (ValueError, "do not fit", lambda: packed(k=k[:5])), (ValueError, "do not fit", lambda: packed(v=k[..., :32])),
+            (ValueError, "contiguous", lambda: packed(q=q.transpose(1, 2))), (TypeError, "dtype", lambda: packed(cu=cu.long())),
+            (ValueError, "batch", lambda: packed(cu=cu[:0])), (ValueError, "entries", lambda: packed(lse=torch.zeros(5, device=DEV))),
+            (TypeError, "dtype", lambda: packed(lse=torch.zeros(24, device=DEV, dtype=BF16))), (HaloError, "workspace", lambda: packed(workspace=slot)),
+            (HaloError, "scale", lambda: packed(scale=0.0)), (HaloError, "strides", lambda: packed(q=torch.zeros(6, 4, 68, dtype=BF16, device=DEV)[..., :64])),
+            (HaloError, "multiple of 8", lambda: packed(q=q[..., :60], k=k[..., :60], v=k[..., :60], out=out[..., :60])),
+            (HaloError, "aligned", lambda: packed(q=torch.zeros(6 * 256 + 1, dtype=BF16, device=DEV)[1:].view(6, 4, 64))),
+            (HaloError, "kv_heads", lambda: packed(k=torch.zeros(6, 3, 64, dtype=BF16, device=DEV), v=torch.zeros(6, 3, 64, dtype=BF16, device=DEV))),
+            (ValueError, "same shape", lambda: paged(v_cache=kc[:2])), (ValueError, "same shape", lambda: paged(v_cache=kc.transpose(1, 2).contiguous().transpose(1, 2))),
+            (TypeError, "q's", lambda: paged(k_cache=kc.half(), v_cache=kc.half())), (ValueError, "do not fit", lambda: paged(table=_i32([[0], [1]]))),
+            (ValueError, "entries", lambda: paged(kv_len=_i32([1, 2]))), (TypeError, "CUDA", lambda: paged(kv_len=None)), (TypeError, "CUDA", lambda: paged(table=table.cpu())),
+            (HaloError, "page size", lambda: paged(k_cache=kc[:, :15], v_cache=kc[:, :15])), (ValueError, "do not fit", lambda: store(k=k[..., :32], v=k[..., :32])),
+            (ValueError, "entries", lambda: store(slot=slot[:5])), (TypeError, "dtype", lambda: store(slot=slot.int())), (TypeError, "k's", lambda: store(v=k.half())),
+            (HaloError, "dtype combination", lambda: store(k_cache=kc.float(), v_cache=kc.float())), (ValueError, "entries", lambda: plan(past=_i32([1, 2]))),
+            (HaloError, "page size", lambda: plan(page_size=17)), (ValueError, "out of range", lambda: plan(page_size=-16)), (TypeError, "integer", lambda: plan(page_size="x")),
+            (ValueError, "entries", lambda: plan(cu=_i32([0]))), (ValueError, "contiguous", lambda: plan(table=torch.zeros(1, dtype=torch.int32, device=DEV).expand(2, 3), past=_i32([0, 0]), fresh=_i32([0, 0]))),
+            (ValueError, "overlap", lambda: plan(table=torch.zeros(1, 3, dtype=torch.int32, device=DEV).expand(2, 3), past=_i32([0, 0]), fresh=_i32([0, 0])))):
+        with pytest.raises(error, match=word):
+            call()
