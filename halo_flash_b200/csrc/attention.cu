@@ -17,9 +17,12 @@
 // ragged batches, and one long sequence that must be split over the whole GPU. No host knowledge of the lengths is
 // needed; every CTA finds its piece from cu / kv_len by itself.
 //
-// Roles in a CTA (384 threads): warp 8 copies Q, K and V by TMA into shared memory (K and V through a ring of
-// stages), one thread of warp 9 issues the tcgen05.mma, warp 10 clears what no row may see of V, warps 0-3 and 4-7 are two softmax groups that take alternate key tiles
-// (thread = row), so that one group's exponentials run beside the other's TMEM traffic and the tensor cores.
+// Roles in a CTA (640 threads): warp 16 copies Q, K and V by TMA into shared memory (K and V through a ring of
+// stages), one thread of warp 17 issues the tcgen05.mma, warp 18 clears what no row may see of V, and warps 0-15 are two
+// pairs of softmax groups. The pairs take alternate key tiles, so that one's exponentials run beside the other's TMEM
+// traffic; in a pair thread = row, each group with half of the tile's keys, and the two trade their maxima. (Two groups
+// with whole rows of 128 held 208 registers a thread and waited for their own latencies: the exponential unit, 16 a clock,
+// was busy 55 % of the time at D = 64.)
 //
 // Waits are bounded as in stage.cuh: one that runs out sets a flag that makes the other waits return at once, the CTA
 // finishes its control flow without storing, and the count is reported by halo_b200_stage_timeouts.
@@ -35,11 +38,11 @@ namespace {
 __device__ unsigned int g_attn_timeouts = 0;
 
 constexpr uint32_t kRows = kAttnRows;
-constexpr uint32_t kThreads = 384;
-// Registers: three warpgroups of 168 at launch; the copying and multiplying one gives 80 a thread to the softmax
-// groups, which hold a whole row of S: 2 x 128 x 208 + 128 x 88 = 384 x 168.
-constexpr uint32_t kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "a share above the launch's total would wait for good");
+constexpr uint32_t kThreads = 640, kSoftmaxWarps = 16;
+// Registers: five warpgroups of 96 at launch; the copying and multiplying one gives 32 a thread to the softmax groups,
+// which hold half a row of S: 4 x 128 x 104 + 128 x 64 = 640 x 96.
+constexpr uint32_t kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
+static_assert(512 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "a share above the launch's total would wait for good");
 constexpr uint32_t kJobCost = 2;   // what a job costs beside its key tiles, in key tiles
 constexpr uint32_t kSnap = 1;      // a border within so many tiles of a job's end moves to that end
 constexpr uint32_t kMinShare = 3;  // least piece of work of a CTA
@@ -56,7 +59,7 @@ struct Shape {
   static constexpr uint32_t kQBytes = kRows * D * 2;
   static constexpr uint32_t kStages = kStageBytes != 32768 ? 8 : D == 256 ? 5 : 4;
   static constexpr uint32_t kKeyRows = kKeys / CG, kVChunks = D / 64 / CG;
-  static constexpr uint32_t kParts = kKeys / 64;                       // P is handed on in parts of 64 keys
+  static constexpr uint32_t kHalf = kKeys / 2;                         // keys of a softmax group, and of a part of P
   // TMEM, 512 columns: buffers of S (which P replaces) from 0, O at the end. With three buffers S(g + 2) is computed while
   // P(g) waits for its product, and neither softmax group waits for S; two leave 128 + 2 x 128 columns at D = 256.
   static constexpr uint32_t kBufs = D <= 128 ? 3 : 2, kAhead = kBufs - 1, kTmemO = 512 - D;
@@ -64,7 +67,8 @@ struct Shape {
   // are finished before the next one's begin.
   static constexpr uint32_t kQBufs = D <= 128 ? 2 : 1;
   static constexpr bool kDrain = kQBufs == 1;
-  static constexpr uint32_t kSlots = kDrain ? 2 : 4;  // references and denominators in flight between the two groups
+  static constexpr uint32_t kSlots = kDrain ? 2 : 4;     // references and denominators in flight between the two pairs
+  static constexpr uint32_t kMaxSlots = kDrain ? 1 : 2;  // maxima in flight between the groups of a pair
 };
 
 struct alignas(16) Basics {
@@ -75,10 +79,11 @@ template <int D, int CG>
 struct alignas(16) Shared : Basics {
   using Sh = Shape<D, CG>;
   unsigned long long kv_full[Sh::kStages], kv_empty[Sh::kStages], q_full[Sh::kQBufs], q_empty[Sh::kQBufs];
-  unsigned long long s_full[Sh::kBufs], p_full[Sh::kBufs][Sh::kParts], pv_done[Sh::kBufs], o_empty, v_dirty, v_clean;
+  unsigned long long s_full[Sh::kBufs], p_full[Sh::kBufs][2], pv_done[Sh::kBufs], o_empty, v_dirty, v_clean;
   unsigned long long m_full[Sh::kSlots][4], l_full[Sh::kSlots][4];
-  float m[Sh::kSlots][kRows];
   float l[Sh::kSlots][kRows];
+  uint16_t m[Sh::kSlots][kRows];            // references, the upper halves of fp32 numbers
+  uint16_t mx[2][Sh::kMaxSlots][2][kRows];  // maxima of a pair's two groups, the same
 };
 template <int D, int CG>
 constexpr uint32_t kSmemBytes =
@@ -182,6 +187,18 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, float (&v)[32]) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_wait_ld16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -203,6 +220,12 @@ __device__ __forceinline__ void tc_wait_ld(float (&v)[N][32]) {
   tc_wait_ld(v[0]);
 #pragma unroll
   for (uint32_t i = 1; i < N; ++i) asm volatile("" : HALO_R32(v[i])::"memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+               "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -447,6 +470,8 @@ __device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+__device__ __forceinline__ float upper(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
+
 template <uint32_t V>
 struct Int {
   static constexpr uint32_t value = V;
@@ -491,10 +516,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t i = 0; i < NQ; ++i) bar_init(&sh.q_full[i], both), bar_init(&sh.q_empty[i], 1);
     bar_init(&sh.v_dirty, 1);
     bar_init(&sh.v_clean, 1);
-    bar_init(&sh.o_empty, 4 * CG);
+    bar_init(&sh.o_empty, 8 * CG);
     for (uint32_t i = 0; i < NB; ++i) {
       bar_init(&sh.s_full[i], 1);
-      for (uint32_t w = 0; w < Sh::kParts; ++w) bar_init(&sh.p_full[i][w], 4 * CG);
+      for (uint32_t w = 0; w < 2; ++w) bar_init(&sh.p_full[i][w], 4 * CG);
       bar_init(&sh.pv_done[i], 1);
     }
     for (uint32_t i = 0; i < NS; ++i)
@@ -502,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == kSoftmaxWarps + 1) {
     if constexpr (CG == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -527,10 +552,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp >= 8) {
+  if (warp >= kSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     Pieces<KT> pc(c, sh, tq);
-    if (warp == 8) {
+    if (warp == kSoftmaxWarps) {
       // ---- copies -------------------------------------------------------------------------------------------------
       uint32_t fill = 0, job = 0;
       uint32_t issued = 0;  // stages that have had a load
@@ -624,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           stage_wait(smem_addr(&sh.q_full[i]), 1);
         }
       }
-    } else if (warp == 9 && rank == 0) {
+    } else if (warp == kSoftmaxWarps + 1 && rank == 0) {
       // ---- matrix products, issued by one thread (of the pair) -----------------------------------------------------
       constexpr uint32_t idesc_s = instr_desc<T>(CG * kRows, KT, false), idesc_o = instr_desc<T>(CG * kRows, D, true);
       const uint32_t qs = uniform(q_smem), kvs = uniform(kv_smem), tm = uniform(tmem);
@@ -648,14 +673,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (v.first && v.job > 0) wait(sh, &sh.o_empty, (v.job - 1) & 1u);
 #pragma unroll
-        for (uint32_t part = 0; part < Sh::kParts; ++part) {
+        for (uint32_t part = 0; part < 2; ++part) {
           wait(sh, &sh.p_full[buf][part], pph);
           tc_after();
           if (elect()) {
 #pragma unroll
-            for (uint32_t k = part * 4; k < part * 4 + 4; ++k)
+            for (uint32_t k = part * (Sh::kHalf / 16); k < (part + 1) * (Sh::kHalf / 16); ++k)
               mma_ts<CG>(tm + Sh::kTmemO, tm + buf * KT + k * 8u, d + k * (2048u >> 4), idesc_o, k == 0 ? acc : 1u);
-            if (part + 1 == Sh::kParts) {
+            if (part == 1) {
               tc_commit<CG>(&sh.kv_empty[st]);
               tc_commit<CG>(&sh.pv_done[buf]);
             }
@@ -698,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t1 > t0) ++job;
       }
       while (left && !aborted(sh)) pv();
-    } else if (warp == 10) {
+    } else if (warp == kSoftmaxWarps + 2) {
       // ---- V rows that no query row sees count with weight 0, but 0 times what stands there may be NaN: they are
       // cleared. And a pair's second CTA tells the leader what has landed.
       uint32_t st = 0, ph = 0, jobs = 0, tails = 0, left = 0;
@@ -765,10 +790,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       else bar_arrive_leader(b);
     };
     // ---- softmax, and the outputs -------------------------------------------------------------------------------
-    const uint32_t wg = warp >> 2, quad = warp & 3u, row = quad * 32u + lane;
+    constexpr uint32_t HK = Sh::kHalf;
+    const uint32_t pair = warp >> 3, half = (warp >> 2) & 1u, quad = warp & 3u, row = quad * 32u + lane;
     const uint32_t lane_base = (quad * 32u) << 16;
     const uint32_t my_tok = row / c.group, my_head = row - my_tok * c.group;
-    uint32_t g = 0, shares = 0;  // tiles so far, jobs in which both groups had a tile
+    // the 64 threads of a pair that share 32 rows
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1u + pair * 4u + quad) : "memory"); };
+    uint32_t g = 0, job = 0;  // tiles so far, pieces with tiles
     if (threadIdx.x == 0 && rank == 0) c.meta[8u * unit] = c.meta[8u * unit + 1] = 0;
     for (; pc.next(); pc.advance()) {
       const uint32_t tok0 = pc.i * tq + rank * tq_cta;
@@ -782,27 +810,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       float before = -INFINITY;       // the one of the tile before
       const uint32_t g0 = g;
       g += pc.t1 - pc.t0;
-      for (uint32_t t = pc.t0 + ((g0 ^ wg) & 1u); t < pc.t1; t += 2) {
+      for (uint32_t t = pc.t0 + ((g0 ^ pair) & 1u); t < pc.t1; t += 2) {
         const uint32_t g = g0 + (t - pc.t0);
         const uint32_t buf = g % NB, slot = g % NS;
         wait(sh, &sh.s_full[buf], (g / NB) & 1u);
         tc_after();
         if (busy) {
-          float s[KT / 32][32];
+          float s[HK / 32][32];
 #pragma unroll
-          for (uint32_t x = 0; x < KT / 32; ++x) tc_ld32(tmem + lane_base + buf * KT + x * 32u, s[x]);
-          float ref = -INFINITY;  // the other group's, of the tile before
+          for (uint32_t x = 0; x < HK / 32; ++x) tc_ld32(tmem + lane_base + buf * KT + half * HK + x * 32u, s[x]);
+          float ref = -INFINITY;  // the other pair's, of the tile before
           if (t > pc.t0) {
             wait(sh, &sh.m_full[(g - 1) % NS][quad], ((g - 1) / NS) & 1u);
-            ref = sh.m[(g - 1) % NS][row];
+            ref = upper(sh.m[(g - 1) % NS][row]);
           }
           before = ref;
           tc_wait_ld(s);
-          const uint32_t key0 = t * KT;
-          if (key0 + KT > min(all_see, pc.keys)) {
+          const uint32_t key0 = t * KT + half * HK;
+          if (key0 + HK > min(all_see, pc.keys)) {
             const uint32_t left = limit > key0 ? limit - key0 : 0u;
 #pragma unroll
-            for (uint32_t x = 0; x < KT / 32; ++x) {
+            for (uint32_t x = 0; x < HK / 32; ++x) {
               const uint32_t over = left > x * 32 ? left - x * 32 : 0u, keep = over >= 32 ? 0xFFFFFFFFu : (1u << over) - 1u;
 #pragma unroll
               for (uint32_t y = 0; y < 32; ++y)
@@ -811,94 +839,107 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains
 #pragma unroll
-          for (uint32_t x = 0; x < KT; x += 2) part[x / 2 % 4] = max3f(part[x / 2 % 4], s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
+          for (uint32_t x = 0; x < HK; x += 2) part[x / 2 % 4] = max3f(part[x / 2 % 4], s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
           float mx = fmaxf(max3f(part[0], part[1], part[2]), part[3]);
           if (row >= rows) mx = -INFINITY;  // no query row: what stands there has no say
+          // The groups trade the upper halves of their maxima: any number near the maximum will do for a reference, as long
+          // as both groups take the same.
+          uint16_t* trade = sh.mx[pair][(g >> 1) % Sh::kMaxSlots][0];
+          trade[half * kRows + row] = static_cast<uint16_t>(__float_as_uint(mx) >> 16);
+          tc_before();  // behind this P of either group may replace S
+          pair_sync();
+          tc_after();
+          mx = fmaxf(upper(trade[row]), upper(trade[kRows + row]));
           // the reference follows where it has fallen too far behind
           const float grown = __fmul_rn(mx - ref, c.scale_log2);
           const bool follow = grown > kLazy;  // also from -inf; false for -inf against -inf (NaN)
           const float next_ref = follow ? mx : ref;
-          if (__any_sync(kFullMask, follow && ref != -INFINITY)) {
+          if (__any_sync(kFullMask, follow && ref != -INFINITY)) {  // in both groups of the pair alike
             wait(sh, &sh.pv_done[(g - 1) % NB], ((g - 1) / NB) & 1u);
             tc_after();
             const float f = follow && ref != -INFINITY ? ex2_approx(-grown) : 1.0f;
 #pragma unroll 1
-            for (uint32_t x = 0; x < D / 32; ++x) {
-              float o[32];
-              tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u, o);
-              tc_wait_ld(o);
-              uint32_t r[32];
+            for (uint32_t x = 0; x < D / 2; x += 16) {
+              uint32_t o[16];
+              tc_ld16(tmem + lane_base + Sh::kTmemO + half * (D / 2) + x, o);
+              tc_wait_ld16(o);
 #pragma unroll
-              for (int y = 0; y < 32; ++y) r[y] = __float_as_uint(__fmul_rn(o[y], f));
-              tc_st32(tmem + lane_base + Sh::kTmemO + x * 32u, r);
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__fmul_rn(__uint_as_float(o[y]), f));
+              tc_st16(tmem + lane_base + Sh::kTmemO + half * (D / 2) + x, o);
             }
             tc_wait_st();
+            tc_before();
+            pair_sync();  // the first part of P is handed on when all columns are done
+            tc_after();
           }
-          sh.m[slot][row] = next_ref;
-          __syncwarp();
-          if (lane == 0) bar_arrive(&sh.m_full[slot][quad]);
+          if (half == 0) {
+            sh.m[slot][row] = static_cast<uint16_t>(__float_as_uint(next_ref) >> 16);
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.m_full[slot][quad]);
+          }
           // p = 2^(c s - c ref); a row that has seen nothing yet has s = -inf everywhere, and 0 does for its reference
           const float mc = next_ref == -INFINITY ? 0.0f : __fmul_rn(next_ref, c.scale_log2);
           const float2 c2 = make_float2(c.scale_log2, c.scale_log2), m2 = make_float2(-mc, -mc);
-          float2 sum = make_float2(0.0f, 0.0f);
+          float2 sum[2] = {};
+          uint32_t r[HK / 2];
 #pragma unroll
-          for (uint32_t x = 0; x < KT / 64; ++x) {
-            uint32_t r[32];
-#pragma unroll
-            for (uint32_t y = 0; y < 32; ++y) {
-              const uint32_t at = x * 64 + 2 * y;
-              float2 v = __ffma2_rn(make_float2(s[at / 32][at % 32], s[at / 32][at % 32 + 1]), c2, m2);
-              v.x = ex2_approx(v.x);
-              v.y = ex2_approx(v.y);
-              sum = __fadd2_rn(sum, v);
-              r[y] = pack2<T>(v.x, v.y);
-            }
-            tc_st32(tmem + lane_base + buf * KT + x * 32u, r);
-            if (x + 1 < Sh::kParts) {  // the first part goes to the tensor cores while the second is computed
-              tc_wait_st();
-              tc_before();
-              __syncwarp();
-              if (lane == 0) tell_leader(&sh.p_full[buf][x]);
-            }
+          for (uint32_t y = 0; y < HK / 2; ++y) {
+            const uint32_t at = 2 * y;
+            float2 v = __ffma2_rn(make_float2(s[at / 32][at % 32], s[at / 32][at % 32 + 1]), c2, m2);
+            v.x = ex2_approx(v.x);
+            v.y = ex2_approx(v.y);
+            sum[y % 2] = __fadd2_rn(sum[y % 2], v);
+            r[y] = pack2<T>(v.x, v.y);
           }
+          if constexpr (HK == 64) tc_st32(tmem + lane_base + buf * KT + half * (HK / 2), r);
+          else tc_st16(tmem + lane_base + buf * KT + half * (HK / 2), r);
           if (next_ref != m) {
             if (m != -INFINITY) l = __fmul_rn(l, ex2_approx(__fmul_rn(m - next_ref, c.scale_log2)));
             m = next_ref;
           }
-          l += sum.x + sum.y;
+          sum[0] = __fadd2_rn(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
           tc_wait_st();
-        } else {
-          if (lane == 0) {
-            bar_arrive(&sh.m_full[slot][quad]);
-            for (uint32_t x = 0; x + 1 < Sh::kParts; ++x) tell_leader(&sh.p_full[buf][x]);
-          }
+        } else if (half == 0 && lane == 0) {
+          bar_arrive(&sh.m_full[slot][quad]);
         }
         tc_before();
         __syncwarp();
-        if (lane == 0) tell_leader(&sh.p_full[buf][Sh::kParts - 1]);
+        if (lane == 0) tell_leader(&sh.p_full[buf][half]);
       }
       const bool any = pc.t1 > pc.t0, whole = pc.t0 == 0 && pc.t1 == pc.n;
-      const bool both_groups = pc.t1 - pc.t0 >= 2;
-      const uint32_t shared = shares % NS, share_phase = (shares / NS) & 1u;
-      if (both_groups) ++shares;
-      // The group of the last tile writes the outputs, while the other one, having left its denominator behind, goes on
-      // to the next job's first tile.
-      const bool owner = any ? ((g - 1) & 1u) == wg : wg == 0;
+      // The pair of the last tile writes the outputs, while the other one, having left its denominator behind, goes on
+      // to the next job's first tile. (No pair is NS jobs ahead of the other: O takes the products of one job at a time.)
+      const bool owner = any ? ((g - 1) & 1u) == pair : pair == 0;
+      float* sl = &sh.l[job % NS][row];
+      unsigned long long* l_full = &sh.l_full[job % NS][quad];
+      const uint32_t l_phase = (job / NS) & 1u;
+      if (any) ++job;
       if (!owner) {
-        if (both_groups) {
-          sh.l[shared][row] = l;
-          __syncwarp();
-          if (lane == 0) bar_arrive(&sh.l_full[shared][quad]);
+        if (any) {
+          if (half == 1) *sl = l;
+          pair_sync();
+          if (half == 0) {
+            *sl += l;
+            __syncwarp();
+            if (lane == 0) bar_arrive(l_full);
+          }
         }
       } else {
         const float ref = m;
-        float total = l;
-        if (both_groups) {
-          wait(sh, &sh.l_full[shared][quad], share_phase);
+        float total = 0.0f;
+        if (any) {
+          wait(sh, l_full, l_phase);
           // over the reference of the tile before the last one
-          const float other = sh.l[shared][row];
-          if (before == ref) total += other;
-          else if (before != -INFINITY) total = __fmaf_rn(other, ex2_approx(__fmul_rn(before - ref, c.scale_log2)), total);
+          const float other = *sl, others = before == ref ? other
+                                            : before == -INFINITY ? 0.0f
+                                                                  : __fmul_rn(other, ex2_approx(__fmul_rn(before - ref, c.scale_log2)));
+          pair_sync();
+          if (half == 1) *sl = l;
+          pair_sync();
+          if (half == 0) *sl = (l + *sl) + others;
+          pair_sync();
+          total = *sl;
         }
         if (any) {
           wait(sh, &sh.pv_done[(g - 1) % NB], ((g - 1) / NB) & 1u);
@@ -916,51 +957,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             out4[y] = reinterpret_cast<T*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(to), (lane & ~3u) + y));
           // The loop stays rolled: unrolled, its first pass is bound by instruction fetches (10000 cycles for 64 KB).
 #pragma unroll 1
-          for (uint32_t x = 0; x < D / 32; x += 2) {
-            float o[2][32];
-            tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u, o[0]);
-            tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u + 32u, o[1]);
+          for (uint32_t x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
+            float o[32];
+            tc_ld32(tmem + lane_base + Sh::kTmemO + x, o);
             tc_wait_ld(o);
+            uint4 u[4];
 #pragma unroll
-            for (uint32_t z = 0; z < 2; ++z) {
-              uint4 u[4];
+            for (uint32_t y = 0; y < 4; ++y) {
+              u[y].x = pack2<T>(__fmul_rn(o[8 * y], inv), __fmul_rn(o[8 * y + 1], inv));
+              u[y].y = pack2<T>(__fmul_rn(o[8 * y + 2], inv), __fmul_rn(o[8 * y + 3], inv));
+              u[y].z = pack2<T>(__fmul_rn(o[8 * y + 4], inv), __fmul_rn(o[8 * y + 5], inv));
+              u[y].w = pack2<T>(__fmul_rn(o[8 * y + 6], inv), __fmul_rn(o[8 * y + 7], inv));
+              if (total == 0.0f) u[y] = make_uint4(0, 0, 0, 0);  // no key (and without tiles O holds anything)
+            }
+            // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
+            // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
+            trade4(u, lane);
+            const uint32_t at = x + (lane & 3u) * 8u;
+            if (at < c.dim) {
 #pragma unroll
-              for (uint32_t y = 0; y < 4; ++y) {
-                u[y].x = pack2<T>(__fmul_rn(o[z][8 * y], inv), __fmul_rn(o[z][8 * y + 1], inv));
-                u[y].y = pack2<T>(__fmul_rn(o[z][8 * y + 2], inv), __fmul_rn(o[z][8 * y + 3], inv));
-                u[y].z = pack2<T>(__fmul_rn(o[z][8 * y + 4], inv), __fmul_rn(o[z][8 * y + 5], inv));
-                u[y].w = pack2<T>(__fmul_rn(o[z][8 * y + 6], inv), __fmul_rn(o[z][8 * y + 7], inv));
-                if (total == 0.0f) u[y] = make_uint4(0, 0, 0, 0);  // no key (and without tiles O holds anything)
-              }
-              // A lane holds 64 bytes of its own row; a store of those would touch 32 lines. Four lanes trade their four
-              // 16-byte parts, so that each store covers 64 bytes of each of eight rows.
-              trade4(u, lane);
-              const uint32_t at = (x + z) * 32u + (lane & 3u) * 8u;
-              if (at < c.dim) {
-#pragma unroll
-                for (uint32_t y = 0; y < 4; ++y)
-                  if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
-              }
+              for (uint32_t y = 0; y < 4; ++y)
+                if (out4[y]) *reinterpret_cast<uint4*>(out4[y] + at) = u[y];
             }
           }
-          if (mine && c.lse)
+          if (mine && c.lse && half == 0)
             c.lse[token * (c.kv_heads * c.group) + head] =
                 total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total)), 0.69314718055994531f);
         } else if (busy) {  // a piece of a split job; pieces have tiles
           float* piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
 #pragma unroll 1
-          for (uint32_t x = 0; x < D / 32; ++x) {
+          for (uint32_t x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
             float o[32];
-            tc_ld32(tmem + lane_base + Sh::kTmemO + x * 32u, o);
+            tc_ld32(tmem + lane_base + Sh::kTmemO + x, o);
             tc_wait_ld(o);
             // [column / 4][row] quads, so that a warp's rows lie side by side
             if (mine) {
 #pragma unroll
               for (uint32_t y = 0; y < 32; y += 4)
-                *reinterpret_cast<float4*>(piece + ((x * 32u + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+                *reinterpret_cast<float4*>(piece + ((x + y) / 4 * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
           }
-          if (mine) {
+          if (mine && half == 0) {
             piece[D * kRows + row] = ref;
             piece[(D + 1) * kRows + row] = total;
           }
@@ -982,7 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_before();
   sync_all<CG>();
   tc_after();
-  if (warp == 9) {
+  if (warp == kSoftmaxWarps + 1) {
     if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
