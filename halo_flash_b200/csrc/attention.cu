@@ -557,55 +557,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     Pieces<KT> pc(c, sh, tq);
     if (warp == kSoftmaxWarps) {
       // ---- copies -------------------------------------------------------------------------------------------------
-      uint32_t fill = 0, job = 0;
+      uint32_t job = 0;
       uint32_t issued = 0;  // stages that have had a load
       const uint32_t q_bytes = tq_cta * c.group * 128u * kChunks;
-      // One operand's tile: up to `kMost` key rows from key0 on, kCh chunks of 64 columns from `col` on, laid out
-      // [chunk][row]. One lane looks up each box's page; an elected thread issues the copies.
-      auto load_kv = [&](auto most, auto chunks, const CUtensorMap* map, uint32_t row0, uint32_t b, uint32_t h, uint32_t key0, uint32_t keys,
-                         uint32_t col, uint32_t seq) {
+      uint32_t st = 0, ph = 1;  // the next stage, and the parity of its kv_empty phase (a new barrier's phase before the first is over)
+      const uint32_t shift = c.box_shift, page_mask = (1u << c.page_shift) - 1u, vcol = uniform(rank * (D / CG));
+      // One operand's tile: up to `kMost` key rows from key0 (of the sequence) on, kCh chunks of 64 columns from `col` on,
+      // laid out [chunk][row], in boxes of rows that lie in one page; lane first + x holds the page of box x. An elected
+      // thread issues the copies.
+      auto load_kv = [&](auto most, auto chunks, const CUtensorMap* map, uint32_t row0, uint32_t h, uint32_t key0, uint32_t keys, uint32_t col,
+                         uint32_t pages, uint32_t first) {
         constexpr uint32_t kMost = decltype(most)::value, kCh = decltype(chunks)::value;
-        const uint32_t st = uniform(seq % ST);
         // rows behind the last visible key are left out by whole boxes
-        const uint32_t rows = keys > key0 ? min(kMost, keys - key0) : 0u, box = c.box_rows;
-        const uint32_t boxes = uniform((rows + box - 1) / box);
-        uint32_t page = 0, row = row0 + key0 + lane * box;
-        if (c.table && lane < boxes) {
-          const uint32_t key = key0 + lane * box;
-          page = static_cast<uint32_t>(c.table[b * c.table_stride + (key >> c.page_shift)]);
-          row = key & ((1u << c.page_shift) - 1u);
-        }
-        if (seq >= ST) wait(sh, &sh.kv_empty[st], (seq / ST - 1) & 1u);
+        const uint32_t rows = keys > key0 ? min(kMost, keys - key0) : 0u, boxes = uniform((rows + (1u << shift) - 1u) >> shift);
+        const uint32_t us = uniform(st), bar = smem_addr(&sh.kv_full[0]) + us * 8u, base = kv_smem + us * Sh::kStageBytes, hh = uniform(h);
+        const uint32_t row = uniform(c.table ? key0 & page_mask : row0 + key0);
+        const uint32_t page0 = __shfl_sync(kFullMask, pages, first), page1 = __shfl_sync(kFullMask, pages, first + 1);
+        wait(sh, &sh.kv_empty[st], ph);
         if (aborted(sh)) return;
         issued |= 1u << st;
-        const uint32_t bar = uniform(smem_addr(&sh.kv_full[st])), base = uniform(kv_smem + st * Sh::kStageBytes);
-        const uint32_t hh = uniform(h);
-        if (elect()) stage_expect(bar, boxes * box * 128u * kCh);
-        __syncwarp();
-        for (uint32_t x = 0; x < boxes; ++x) {
-          const uint32_t r = __shfl_sync(kFullMask, row, x), pg = __shfl_sync(kFullMask, page, x), to = base + uniform(x * box * 128u);
-          if (elect()) {
+        auto box = [&](uint32_t x, uint32_t r, uint32_t page) {
 #pragma unroll
-            for (uint32_t ch = 0; ch < kCh; ++ch)
-              tma_4d(to + ch * kMost * 128u, map, static_cast<int>(col + ch * 64), static_cast<int>(r), static_cast<int>(hh), static_cast<int>(pg), bar);
-          }
+          for (uint32_t ch = 0; ch < kCh; ++ch)
+            tma_4d(base + (ch * kMost + (x << shift)) * 128u, map, static_cast<int>(col + ch * 64), static_cast<int>(r), static_cast<int>(hh),
+                   static_cast<int>(page), bar);
+        };
+        if (elect()) {
+          stage_expect(bar, (boxes << shift) * 128u * kCh);
+          if (boxes > 0) box(0, row, page0);
+          if (boxes > 1) box(1, c.table ? (row + (1u << shift)) & page_mask : row + (1u << shift), page1);
+        }
+        __syncwarp();
+        for (uint32_t x = 2; x < boxes; ++x) {  // pages of less than 64 rows
+          const uint32_t page = __shfl_sync(kFullMask, pages, first + x), r = c.table ? (row + (x << shift)) & page_mask : row + (x << shift);
+          if (elect()) box(x, r, page);
           __syncwarp();
         }
+        if (++st == ST) st = 0, ph ^= 1u;
+      };
+      // Each lane looks up the page of one box of a tile, a tile ahead of its use.
+      auto look_up = [&](uint32_t t) -> uint32_t {
+        const uint32_t key = t * KT + (lane << shift);
+        return c.table && key < min(pc.keys, (t + 1) * KT) ? static_cast<uint32_t>(c.table[pc.b * c.table_stride + (key >> c.page_shift)]) : 0u;
       };
       // The order of use, which is also the order of the stages: K(g), V(g - kAhead), ..., what is left of V at the end
       // (and, where Q has one buffer, at the end of each job).
       struct Tile {
-        uint32_t row0, b, h, t, keys;
+        uint32_t row0, h, t, keys, pages;
       } last[Sh::kAhead];
       uint32_t left = 0;  // tiles whose V is still to come
-      const uint32_t vcol = uniform(rank * (D / CG));
       auto load_v = [&] {
         const Tile& v = left == 1 ? last[0] : last[Sh::kAhead - 1];
-        load_kv(Int<KT>{}, Int<Sh::kVChunks>{}, &vmap, v.row0, v.b, v.h, v.t * KT, v.keys, vcol, fill++);
+        load_kv(Int<KT>{}, Int<Sh::kVChunks>{}, &vmap, v.row0, v.h, v.t * KT, v.keys, vcol, v.pages, 0);
         --left;
       };
       for (; pc.next() && !aborted(sh); pc.advance()) {
+        uint32_t ahead = pc.t0 < pc.t1 ? look_up(pc.t0) : 0u;
         for (uint32_t t = pc.t0; t < pc.t1; ++t) {
+          const uint32_t pages = ahead;
+          if (t + 1 < pc.t1) ahead = look_up(t + 1);
           if (t == pc.t0) {
             if constexpr (Sh::kDrain)
               while (left) load_v();
@@ -623,18 +633,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             ++job;
           }
-          load_kv(Int<Sh::kKeyRows>{}, Int<kChunks>{}, &kmap, pc.s.row0, pc.b, pc.h, t * KT + rank * Sh::kKeyRows, pc.keys, 0, fill++);
+          load_kv(Int<Sh::kKeyRows>{}, Int<kChunks>{}, &kmap, pc.s.row0, pc.h, t * KT + rank * Sh::kKeyRows, pc.keys, 0, pages,
+                  rank * (Sh::kKeyRows >> shift));
           if (left == Sh::kAhead) load_v();
 #pragma unroll
           for (uint32_t i = Sh::kAhead - 1; i > 0; --i) last[i] = last[i - 1];
-          last[0] = Tile{pc.s.row0, pc.b, pc.h, t, pc.keys};
+          last[0] = Tile{pc.s.row0, pc.h, t, pc.keys, pages};
           ++left;
         }
       }
       while (left && !aborted(sh)) load_v();
       // every stage's last use is over before the CTA may leave: no arrival of the other CTA's products is under way
       if (!aborted(sh)) {
-        for (uint32_t i = fill > ST ? fill - ST : 0u; i < fill; ++i) wait(sh, &sh.kv_empty[i % ST], (i / ST) & 1u);
+        for (uint32_t i = 0; i < ST; ++i) {
+          wait(sh, &sh.kv_empty[st], ph);
+          if (++st == ST) st = 0, ph ^= 1u;
+        }
         for (uint32_t i = job > NQ ? job - NQ : 0u; i < job; ++i) wait(sh, &sh.q_empty[i % NQ], (i / NQ) & 1u);
       }
       if (aborted(sh)) {
@@ -877,6 +891,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.m_full[slot][quad]);
           }
+          // The other pair waits for that: without this the compiler puts it behind the exponentials, and the pairs take
+          // turns instead of overlapping (2000 instead of 1400 cycles a tile at D = 64).
+#pragma unroll
+          for (uint32_t x = 0; x < HK / 32; ++x) asm volatile("" : HALO_R32(s[x])::"memory");
           // p = 2^(c s - c ref); a row that has seen nothing yet has s = -inf everywhere, and 0 does for its reference
           const float mc = next_ref == -INFINITY ? 0.0f : __fmul_rn(next_ref, c.scale_log2);
           const float2 c2 = make_float2(c.scale_log2, c.scale_log2), m2 = make_float2(-mc, -mc);
@@ -1260,7 +1278,7 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   c.meta = static_cast<uint32_t*>(a.workspace);
   c.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kMetaBytes);
   const uint32_t tq_cta = kRows / c.group, tq = CG * tq_cta;
-  c.box_rows = a.table && (1u << a.page_shift) < 64u ? 1u << a.page_shift : 64u;
+  c.box_shift = a.table && a.page_shift < 6u ? a.page_shift : 6u;
 
   CUtensorMap qm, km, vm;
   const uint64_t qd[3] = {a.dim, a.q_heads, a.tokens}, qs[3] = {1, a.q_head, a.q_row};
@@ -1270,7 +1288,7 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   const uint64_t rows = a.table ? uint64_t{1} << a.page_shift : a.tokens, pages = a.table ? a.pages : 1;
   const uint64_t kd[4] = {a.dim, rows, a.kv_heads, pages};
   const uint64_t ks[4] = {1, a.k_row, a.k_head, a.k_page}, vs[4] = {1, a.v_row, a.v_head, a.v_page};
-  const uint32_t kb[4] = {64, c.box_rows, 1, 1};
+  const uint32_t kb[4] = {64, 1u << c.box_shift, 1, 1};
   e = MakeMap(&km, a.dtype, a.k, 4, kd, ks, kb);
   if (e == cudaSuccess) e = MakeMap(&vm, a.dtype, a.v, 4, kd, vs, kb);
   if (e != cudaSuccess) return e;

@@ -19,7 +19,7 @@ struct AttnCall {
   uint64_t table_stride;
   uint32_t table_cols, page_shift;
   uint32_t batch, tokens, kv_heads, group, dim;
-  uint32_t box_rows;       // key rows of one copy: min(page size, 64)
+  uint32_t box_shift;      // key rows of one copy: min(page size, 64), as a power of two
   int causal;
   float scale_log2;        // softmax scale * log2(e)
   void* out;
