@@ -1595,6 +1595,9 @@ int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table
   REQUIRE(n_free == 0 || free_pages, "%s: the free list is null", what);
   REQUIRE(n_free < (1u << 31) && tokens < (1u << 31), "%s: more than 2^31 pages or tokens", what);
   REQUIRE(table_stride >= table_cols || batch <= 1, "%s: table rows overlap", what);
+  // every CTA reads the lengths while one writes kv_len and cu
+  REQUIRE(batch == 0 || ((kv_len == nullptr || (kv_len != past && kv_len != fresh)) && (cu == nullptr || (cu != past && cu != fresh))),
+          "%s: an output must not be the memory of past or fresh", what);
   REQUIRE(Aligned(table, 4) && Aligned(past, 4) && Aligned(fresh, 4) && Aligned(free_pages, 4) && Aligned(slot, 8) &&
               Aligned(pos, 4) && Aligned(cu, 4) && Aligned(kv_len, 4) && Aligned(status, 4),
           "%s: pointer not aligned to its element type", what);

@@ -57,7 +57,7 @@ struct Shape {
   static constexpr uint32_t kKeys = D == 256 && CG == 1 ? 64 : 128;    // keys of a tile
   static constexpr uint32_t kStageBytes = kKeys * D * 2 / CG;          // one CTA's share of a tile of K or V
   static constexpr uint32_t kQBytes = kRows * D * 2;
-  static constexpr uint32_t kStages = kStageBytes != 32768 ? 8 : D == 256 ? 5 : 4;
+  static constexpr uint32_t kStages = kStageBytes == 32768 ? 4 : 8;
   static constexpr uint32_t kKeyRows = kKeys / CG, kVChunks = D / 64 / CG;
   static constexpr uint32_t kHalf = kKeys / 2;                         // keys of a softmax group, and of a part of P
   // TMEM, 512 columns: buffers of S (which P replaces) from 0, O at the end. With three buffers S(g + 2) is computed while
@@ -82,8 +82,8 @@ struct alignas(16) Shared : Basics {
   unsigned long long s_full[Sh::kBufs], p_full[Sh::kBufs][2], pv_done[Sh::kBufs], o_empty, v_dirty, v_clean;
   unsigned long long m_full[Sh::kSlots][4], l_full[Sh::kSlots][4];
   float l[Sh::kSlots][kRows];
-  uint16_t m[Sh::kSlots][kRows];            // references, the upper halves of fp32 numbers
-  uint16_t mx[2][Sh::kMaxSlots][2][kRows];  // maxima of a pair's two groups, the same
+  float m[Sh::kSlots][kRows];            // references
+  float mx[2][Sh::kMaxSlots][2][kRows];  // maxima of a pair's two groups
 };
 template <int D, int CG>
 constexpr uint32_t kSmemBytes =
@@ -277,7 +277,7 @@ __device__ __forceinline__ Seq load_seq(const AttnCall& c, uint32_t b, uint32_t 
   s.len = s.rows;
   if (c.kv_len) {
     const unsigned long long room = static_cast<unsigned long long>(c.table_cols) << c.page_shift;
-    s.len = static_cast<uint32_t>(min(static_cast<unsigned long long>(c.kv_len[b]), min(room, 0x7FFFFFFFull)));
+    s.len = static_cast<uint32_t>(min(static_cast<unsigned long long>(c.kv_len[b]), min(room, 0x7FFF0000ull)));
   }
   s.off = static_cast<int>(s.len) - static_cast<int>(s.rows);
   s.tiles = (s.rows + tq - 1) / tq;
@@ -469,8 +469,6 @@ __device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-
-__device__ __forceinline__ float upper(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
 
 template <uint32_t V>
 struct Int {
@@ -836,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float ref = -INFINITY;  // the other pair's, of the tile before
           if (t > pc.t0) {
             wait(sh, &sh.m_full[(g - 1) % NS][quad], ((g - 1) / NS) & 1u);
-            ref = upper(sh.m[(g - 1) % NS][row]);
+            ref = sh.m[(g - 1) % NS][row];
           }
           before = ref;
           tc_wait_ld(s);
@@ -856,14 +854,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (uint32_t x = 0; x < HK; x += 2) part[x / 2 % 4] = max3f(part[x / 2 % 4], s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
           float mx = fmaxf(max3f(part[0], part[1], part[2]), part[3]);
           if (row >= rows) mx = -INFINITY;  // no query row: what stands there has no say
-          // The groups trade the upper halves of their maxima: any number near the maximum will do for a reference, as long
-          // as both groups take the same.
-          uint16_t* trade = sh.mx[pair][(g >> 1) % Sh::kMaxSlots][0];
-          trade[half * kRows + row] = static_cast<uint16_t>(__float_as_uint(mx) >> 16);
+          float* trade = sh.mx[pair][(g >> 1) % Sh::kMaxSlots][0];
+          trade[half * kRows + row] = mx;
           tc_before();  // behind this P of either group may replace S
           pair_sync();
           tc_after();
-          mx = fmaxf(upper(trade[row]), upper(trade[kRows + row]));
+          mx = fmaxf(trade[row], trade[kRows + row]);
           // the reference follows where it has fallen too far behind
           const float grown = __fmul_rn(mx - ref, c.scale_log2);
           const bool follow = grown > kLazy;  // also from -inf; false for -inf against -inf (NaN)
@@ -887,13 +883,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_after();
           }
           if (half == 0) {
-            sh.m[slot][row] = static_cast<uint16_t>(__float_as_uint(next_ref) >> 16);
+            sh.m[slot][row] = next_ref;
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.m_full[slot][quad]);
-            // The other pair waits for that. Reading the number back makes the exponentials depend on it; without that the
+            // The other pair waits for that. Reading the reference back makes the exponentials depend on it; without that the
             // assembler puts the arrival behind them, and the pairs take turns instead of overlapping (1900 instead of
             // 1400 cycles a tile at D = 64).
-            next_ref = upper(*static_cast<volatile uint16_t*>(&sh.m[slot][row]));
+            next_ref = *static_cast<volatile float*>(&sh.m[slot][row]);
           }
           // p = 2^(c s - c ref); a row that has seen nothing yet has s = -inf everywhere, and 0 does for its reference
           const float mc = next_ref == -INFINITY ? 0.0f : __fmul_rn(next_ref, c.scale_log2);

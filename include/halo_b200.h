@@ -445,7 +445,7 @@ int halo_b200_conv_step(halo_b200_stream stream, const float* in, float* state, 
                         uint32_t channels, uint32_t kern, char* err, size_t errlen);
 
 /* No counterpart in the reference. The persistent kernels of the library (the conv + SiLU + L2 norm and the fused
- * norm + RoPE at streaming sizes) stage their input rows in shared memory with bulk asynchronous copies and wait
+ * norm + RoPE at streaming sizes, attention) stage their input rows in shared memory with asynchronous copies and wait
  * for them on a barrier object for a bounded time (about a second); a CTA whose wait ran out (never
  * observed) returns without writing its remaining output tiles and is counted. halo_b200_stage_timeouts reads the
  * count (this call synchronizes the device). A non-zero count means the outputs of the calls made before it are
@@ -513,7 +513,8 @@ int halo_b200_scale_silu(halo_b200_stream stream, const float* x, void* y, int y
  * A request that needs more than table_cols pages, or whose pages would pass the end of the free list, is refused: it
  * takes no page, its slots are -1 and its kv_len stays past[r]. Requests are served in order: once the list cannot
  * serve one, it serves none behind it that needs a page. slot and pos have `tokens` entries: those behind the last
- * new token get -1 and 0, new tokens beyond them get none. batch <= 16384, n_free < 2^31, lengths < 2^31. */
+ * new token get -1 and 0, new tokens beyond them get none. batch <= 16384, n_free < 2^31, lengths < 2^31. No output may
+ * lie in the memory of past, fresh or free_pages (a step's kv_len goes to a second buffer). */
 int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table_stride, uint32_t table_cols,
                          const uint32_t* past, const uint32_t* fresh, const int32_t* free_pages, uint32_t n_free,
                          uint32_t page_size, int64_t* slot, uint32_t* pos, uint32_t* cu, uint32_t* kv_len,

@@ -56,7 +56,7 @@ def test_plan_and_store_refuse():
         [table, stride, cols, past, fresh, free, n_free, page, slot, pos, cu, kv, st, batch, tokens]  # noqa: E731
     for change, word in (({"page": 65}, "page size"), ({"table": None}, "table"), ({"past": None}, "null"), ({"fresh": None}, "null"),
                          ({"slot": None}, "slot"), ({"free": None}, "free list"), ({"stride": 3}, "overlap"), ({"batch": 16385}, "16384"),
-                         ({"slot": A + 4}, "aligned"), ({"st": A + 1}, "aligned"), ({"n_free": 1 << 31}, "2^31")):
+                         ({"slot": A + 4}, "aligned"), ({"st": A + 1}, "aligned"), ({"n_free": 1 << 31}, "2^31"), ({"kv": A}, "must not be"), ({"cu": A}, "must not be")):
         assert word in _fails("paged_plan", *plan(**change))
     store = lambda k=A, kr=128, kh=64, v=A, vr=128, vh=64, dt=2, kc=A, vc=A, ct=2, ps=8192, rs=128, hs=64, pages=3, page=64, slot=A, heads=2, d=64, tokens=5: \
         [k, kr, kh, v, vr, vh, dt, kc, vc, ct, ps, rs, hs, pages, page, slot, heads, d, tokens]  # noqa: E731

@@ -306,3 +306,62 @@ def test_tensor_refusals():
             (ValueError, "overlap", lambda: plan(table=torch.zeros(1, 3, dtype=torch.int32, device=DEV).expand(2, 3), past=_i32([0, 0]), fresh=_i32([0, 0])))):
         with pytest.raises(error, match=word):
             call()
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (8, 2, 128), (8, 1, 256), (2, 2, 256)])
+def test_scores_far_from_zero(hq, hk, d):
+    """Scaled scores near -900 and near +900: the softmax is the one of their differences, whatever the type of P."""
+    for sign in (-1.0, 1.0):
+        g = _gen(18)
+        n = 400
+        q, k, v = (_randn(g, n, h, d, dtype=F16) for h in (hq, hk, hk))
+        q[..., 0] = 90.0
+        k[..., 0] = sign * 10.0 * d ** 0.5
+        out, lse = torch.empty_like(q), torch.empty(n, hq, device=DEV)
+        ops.attention_packed(q, k, v, _i32([0, n]), out, lse=lse)
+        o, a, want = exact_rows(q, k, v, True, d ** -0.5)
+        # fp32 sums of terms up to 900 sqrt(d), at most 16 of them rounded at 2^-23: scores are off by up to 16 * 900 * 2^-23
+        # = 2^-9.2, so are p relative to each other
+        bad = ~((out.double() - o).abs() <= 2.0 ** -11 * (o.abs() + a) + 2.0 ** -8 * a + n * 2.0 ** -25 * 6.0)
+        assert not bad.any(), (sign, int(bad.sum()))
+        assert (lse.double() - want).abs().max() < 900 * 2.0 ** -17
+
+
+def test_table_entries_outside_the_cache_read_as_zeros():
+    g, hq, hk, d, page = _gen(19), 8, 2, 128, 16
+    kc, vc = (_randn(g, 6, page, hk, d, dtype=BF16) for _ in range(2))
+    table, n = _i32([[3, -1, 0, 6, 0x7FFFFFFF, 5]]), 6 * page - 5
+    q = _randn(g, 3, hq, d, dtype=BF16)
+    out = torch.empty_like(q)
+    ops.attention_paged(q, kc, vc, table, _i32([n]), _i32([0, 3]), out)
+    zeros = torch.zeros_like(kc[0])
+    k, v = (torch.cat([c[3], zeros, c[0], zeros, zeros, c[5]])[:n] for c in (kc, vc))
+    check(out, None, exact_rows(q, k, v, True, d ** -0.5), BF16, n, 6.0, "outside")
+
+
+def test_large_batches_of_short_sequences():
+    """More sequences than a warp scans at once, some empty, beside one long one; and the same as single tokens over pages."""
+    g, hq, hk, d = _gen(20), 4, 2, 64
+    lens = [(i * 7) % 5 for i in range(400)]
+    lens[200] = 900
+    packed(lens, hq, hk, d, F16, seed=21)
+    past = [(i * 37) % 200 for i in range(300)]
+    past[17] = 4000
+    paged(past, [1] * 300, hq, hk, d, 16, F16, seed=22)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU, each with a workspace of its own (from torch's allocator, as by default)."""
+    g, d = _gen(23), 128
+    sets = [tuple(_randn(g, 1500, h, d, dtype=BF16) for h in (8, 2, 2)) for _ in range(4)]
+    cu = _i32([0, 1500])
+    alone = [ops.attention_packed(q, k, v, cu, torch.empty_like(q)) for q, k, v in sets]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in sets], [torch.full_like(s[0], float("nan")) for s in sets]
+    for _ in range(5):
+        for s, (q, k, v), out in zip(streams, sets, outs):
+            with torch.cuda.stream(s):
+                ops.attention_packed(q, k, v, cu, out)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, outs):
+        assert torch.equal(a, b)

@@ -45,7 +45,7 @@ def run_plan(table, past, fresh, free, page, tokens):
 
 
 @pytest.mark.parametrize("batch,page,cols,most,free,slack", [
-    (1, 16, 4, 30, 10, 0), (8, 64, 40, 1000, 200, 3), (33, 8, 30, 100, 600, 0), (700, 16, 64, 300, 40000, 50), (3000, 256, 8, 600, 9000, 0),
+    (1, 16, 4, 30, 10, 0), (8, 64, 40, 1000, 200, 3), (33, 8, 30, 100, 600, 0), (700, 16, 64, 300, 40000, 50), (3000, 256, 8, 600, 9000, 0), (16384, 16, 3, 20, 30000, 7),
     (20, 16, 8, 80, 30, 5),      # the free list ends
     (20, 16, 3, 40, 300, -40),   # some need more pages than a table row has; fewer slots than tokens
     (5, 32, 4, 50, 0, 0),        # no free page at all
