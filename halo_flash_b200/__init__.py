@@ -3,7 +3,7 @@ elementwise path, behind the C ABI declared in include/halo_b200.h.
 
     csrc/      the kernels and the C ABI (built in-tree into libhalo_b200.so)
     _lib.py    ctypes binding of every entry point
-    ops.py     the five op groups on torch CUDA tensors
+    ops.py     the five op groups, the paged K/V cache and attention on torch CUDA tensors
     device.py  a CUDA stand-in for the reference's rt::Device (launch by kernel name)
     chain.py   the per-layer op chain (36 DeltaNet + 12 GQA layers) and its token sharding
 

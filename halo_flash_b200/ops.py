@@ -1,4 +1,4 @@
-"""Tensor-level front end of the C ABI: the five op groups on torch CUDA tensors.
+"""Tensor-level front end of the C ABI: the five op groups, the paged K/V cache and attention on torch CUDA tensors.
 
 torch is plumbing here (device memory and the current stream); every function
 forwards to one `halo_b200_*` entry point of libhalo_b200.so and nothing else.

@@ -148,3 +148,36 @@ def test_a_conversation_step_by_step():
             ks, vs = (torch.cat([s[x] for s in seen[b]]) for x in (0, 1))
             check(out[a:e], None, exact_rows(q[a:e], ks, vs, True, d ** -0.5), BF16, ks.shape[0], 7.0, f"session {b} after {fresh}")
         past = kv_len
+
+
+def test_a_layer_step_with_rotation():
+    """plan -> rotation table at the planned positions -> norm + RoPE of Q and K -> store -> attention, on one stream
+    without a look at the device in between; the attention of the rotated rows against 64 bits."""
+    g, hq, hk, d, page = _gen(5), 16, 2, 256, 64
+    past, fresh = [300, 0, 77], [1, 40, 1]
+    t, pages = sum(fresh), 24
+    table = torch.full((3, 8), -1, dtype=torch.int32, device=DEV)
+    ids = torch.randperm(pages, generator=g, device=DEV).to(torch.int32)
+    at = 0
+    for r, p in enumerate(past):
+        n = -(-p // page)
+        table[r, :n] = ids[at:at + n]
+        at += n
+    kc, vc = (_randn(g, pages, page, hk, d, dtype=BF16) for _ in range(2))
+    slot, pos, cu, kv_len = torch.empty(t, dtype=torch.int64, device=DEV), _i32([0] * t), _i32([0] * 4), _i32([0] * 3)
+    ops.paged_plan(table, _i32(past), _i32(fresh), ids[at:], page, slot, pos=pos, cu=cu, kv_len=kv_len)
+    q, k, v = (_randn(g, t, h, d, dtype=BF16) for h in (hq, hk, hk))
+    rot = torch.empty(t, 64, device=DEV)
+    ops.rope_table(rot, 64, 1e7, params=pos, pstride=1)
+    w = torch.zeros(d, device=DEV)
+    before = k.clone()
+    ops.norm_rope_qk_table(q, k, w, w, 1e-6, 64, rot)
+    ops.paged_store(k, v, kc, vc, slot)
+    out = torch.empty_like(q)
+    ops.attention_paged(q, kc, vc, table, kv_len, cu, out)
+    assert pos.tolist() == [300] + list(range(40)) + [77] and not torch.equal(before, k)
+    for b, (p, n) in enumerate(zip(past, fresh)):
+        a = sum(fresh[:b])
+        ks, vs = (c[table[b].long()].flatten(0, 1)[:p + n] for c in (kc, vc))
+        assert torch.equal(ks[p:], k[a:a + n]) and torch.equal(vs[p:], v[a:a + n])
+        check(out[a:a + n], None, exact_rows(q[a:a + n], ks, vs, True, d ** -0.5), BF16, p + n, 7.0, f"request {b}")
