@@ -1086,7 +1086,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
     }
   }
   const uint32_t pieces = last - first + 1;
-  const uint32_t group = blockIdx.y % (4 * CG), rank = group >> 2, row = (group & 3u) * 32u + lane;
+  // the first rows' blocks are the first of the grid: of a single token's tile no others have work
+  const uint32_t parts = gridDim.y / (4 * CG), group = blockIdx.y / parts, rank = group >> 2, row = (group & 3u) * 32u + lane;
   // piece 0 opened the job, the others are what the units behind began with
   auto piece = [&](uint32_t p) { return c.part + ((2ull * (first + p) + (p == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D); };
   const uint4 job = *reinterpret_cast<const uint4*>(c.meta + 8u * first);  // ., ., first token, tokens
@@ -1098,7 +1099,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
   const uint64_t token = job.z + tok0 + row / c.group;
   const uint32_t head = h * c.group + row % c.group;
   T* out = static_cast<T*>(c.out) + token * c.out_row + head * c.out_head;
-  const uint32_t parts = gridDim.y / (4 * CG), quads = D / 4 / parts, q0 = blockIdx.y / (4 * CG) * quads;
+  const uint32_t quads = D / 4 / parts, q0 = (blockIdx.y - group * parts) * quads;
   auto finish2 = [&](uint32_t q, const float4 (&sum)[2], float inv) {  // two quads, q even
     if (mine && q * 4 < c.dim) {
       uint4 u;
@@ -1110,7 +1111,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
     }
   };
   auto finish_lse = [&](float top, float total) {
-    if (c.lse && blockIdx.y < 4 * CG && warp == 0 && mine)
+    if (c.lse && q0 == 0 && warp == 0 && mine)
       c.lse[token * (c.kv_heads * c.group) + head] =
           total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total)), 0.69314718055994531f);
   };
@@ -1172,7 +1173,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
   auto ref = [&](uint32_t p) { return mine ? piece(p)[D * kRows + row] : -INFINITY; };
   float top = -INFINITY, total = 0.0f;
 #pragma unroll 4
-  for (uint32_t p = warp; p < pieces; p += kJoinWarps) top = fmaxf(top, ref(p));
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
+    top = fmaxf(top, ref(p));
+  }
   meet[warp][lane] = top;
   __syncthreads();
 #pragma unroll
@@ -1320,8 +1323,10 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   // jobs of one tile are never split
   if (e != cudaSuccess || tiles <= 1 || units == 1) return e;
   const uint32_t x = static_cast<uint32_t>(jobs < units ? jobs : units);
+  // one wave of blocks with work: a pair's tiles are mostly full, a single CTA's mostly hold 32 rows at most
+  const uint32_t groups = CG == 2 ? 8 : 1;
   uint32_t parts = 1;
-  while (parts < D / 16 && x * 4 * CG * parts * 2 <= static_cast<uint32_t>(sms) * kJoinResident) parts *= 2;
+  while (parts < D / 16 && x * groups * parts * 2 <= static_cast<uint32_t>(sms) * kJoinResident) parts *= 2;
   return LaunchKernel(attention_join_kernel<T, D, CG>, dim3(x, 4 * CG * parts), kJoinWarps * 32, 0, s, c, static_cast<uint32_t>(units));
 }
 
