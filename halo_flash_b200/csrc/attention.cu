@@ -28,6 +28,8 @@
 // finishes its control flow without storing, and the count is reported by halo_b200_stage_timeouts.
 #include "attention.cuh"
 
+#include <atomic>
+
 #include "common.cuh"
 #include "stage.cuh"
 
@@ -43,9 +45,11 @@ constexpr uint32_t kThreads = 640, kSoftmaxWarps = 16;
 // which hold half a row of S: 4 x 128 x 104 + 128 x 64 = 640 x 96.
 constexpr uint32_t kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
 static_assert(512 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "a share above the launch's total would wait for good");
-constexpr uint32_t kJobCost = 2;   // what a job costs beside its key tiles, in key tiles
+// What a job costs beside its key tiles, in key tiles (4096 tokens, 16/2 heads of 256: 121 us with 1, 115 with 2, 116 with 3, 117 with 4).
+constexpr uint32_t kJobCost = 2;
 constexpr uint32_t kSnap = 1;      // a border within so many tiles of a job's end moves to that end
-constexpr uint32_t kMinShare = 3;  // least piece of work of a CTA
+// Least share of a unit, job costs counted (one token over 1501 keys: 15.2 us with 1, 14.9 with 2, 14.2 with 3, 14.9 with 4).
+constexpr uint32_t kMinShare = 3;
 constexpr uint32_t kMaxCtas = 148;
 constexpr float kLazy = 8.0f;      // log2 of the growth that a reference may lag behind
 
@@ -1173,9 +1177,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
   auto ref = [&](uint32_t p) { return mine ? piece(p)[D * kRows + row] : -INFINITY; };
   float top = -INFINITY, total = 0.0f;
 #pragma unroll 4
-  for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
-    top = fmaxf(top, ref(p));
-  }
+  for (uint32_t p = warp; p < pieces; p += kJoinWarps) top = fmaxf(top, ref(p));
   meet[warp][lane] = top;
   __syncthreads();
 #pragma unroll
@@ -1298,6 +1300,16 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(attention_kernel<T, D, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes<D, CG>));
   if (e != cudaSuccess) return e;
+  // setmaxnreg hands on what the launch has: with fewer registers a thread than the shares were added up for, the softmax
+  // groups would wait for good
+  static std::atomic<bool> checked{false};
+  if (!checked.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes f;
+    e = cudaFuncGetAttributes(&f, attention_kernel<T, D, CG>);
+    if (e != cudaSuccess) return e;
+    if (f.numRegs != static_cast<int>(kLaunchRegs)) return cudaErrorInvalidConfiguration;
+    checked.store(true, std::memory_order_relaxed);
+  }
   const uint64_t most_keys = a.table ? static_cast<uint64_t>(a.table_cols) << a.page_shift : a.tokens;
   const uint64_t jobs = (static_cast<uint64_t>(a.tokens) / tq + a.batch) * a.kv_heads;  // at most
   const uint64_t tiles = (most_keys + Shape<D, CG>::kKeys - 1) / Shape<D, CG>::kKeys;
