@@ -52,6 +52,9 @@ constexpr uint32_t kSnap = 1;      // a border within so many tiles of a job's e
 constexpr uint32_t kMinShare = 3;
 constexpr uint32_t kMaxCtas = 148;
 constexpr float kLazy = 8.0f;      // log2 of the growth that a reference may lag behind
+// log2 of a factor on all p, which l has too: in fp16 a p far below the maximum would be subnormal, and 2^(8 + 6) still fits.
+template <typename T>
+constexpr float kLift = __is_same(T, f16) ? 6.0f : 0.0f;
 
 // CG CTAs (a pair of neighbouring SMs, or one) work on a tile of CG x 128 rows. A pair's tensor cores share the
 // operands: each CTA stages half of K (its keys) and half of V (its columns), which halves both the traffic from L2 and
@@ -897,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // p = 2^(c s - c ref); a row that has seen nothing yet has s = -inf everywhere, and 0 does for its reference
           const float mc = next_ref == -INFINITY ? 0.0f : __fmul_rn(next_ref, c.scale_log2);
-          const float2 c2 = make_float2(c.scale_log2, c.scale_log2), m2 = make_float2(-mc, -mc);
+          const float2 c2 = make_float2(c.scale_log2, c.scale_log2), m2 = make_float2(kLift<T> - mc, kLift<T> - mc);
           float2 sum[2] = {};
           uint32_t r[HK / 2];
 #pragma unroll
@@ -1000,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (mine && c.lse && half == 0)
             c.lse[token * (c.kv_heads * c.group) + head] =
-                total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total)), 0.69314718055994531f);
+                total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(ref, c.scale_log2, __log2f(total) - kLift<T>), 0.69314718055994531f);
         } else if (busy) {  // a piece of a split job; pieces have tiles
           float* piece = c.part + ((2ull * unit + (pc.t0 == 0 ? 1u : 0u)) * CG + rank) * AttnPieceFloats(D);
 #pragma unroll 1
@@ -1117,7 +1120,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
   auto finish_lse = [&](float top, float total) {
     if (c.lse && q0 == 0 && warp == 0 && mine)
       c.lse[token * (c.kv_heads * c.group) + head] =
-          total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total)), 0.69314718055994531f);
+          total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total) - kLift<T>), 0.69314718055994531f);
   };
   // a piece that saw nothing (weight 0) says nothing, whatever its sums are
   auto add = [](float4& sum, float w, float4 v) {

@@ -365,3 +365,26 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for a, b in zip(alone, outs):
         assert torch.equal(a, b)
+
+
+def test_many_small_weights_in_fp16():
+    """One key with weight 1 and 60000 with 2^-17 each, whose sum is what the result mostly is: P of these is far below the
+    smallest normal fp16 relative to the maximum."""
+    g, d, n = _gen(24), 64, 60000
+    q, k, v = (_randn(g, r, 1, d, dtype=F16) for r in (1, n, n))
+    q[...] = 0.0
+    q[..., 0] = 8.0
+    k[...] = 0.0
+    k[7, 0, 0] = 17 * 0.6931471805599453  # q k d^-0.5 = 17 ln 2
+    v += 1.0
+    page = 64
+    pages = -(-n // page)
+    kc, vc = (torch.zeros(pages, page, 1, d, dtype=F16, device=DEV) for _ in range(2))
+    kc.view(-1, 1, d)[:n], vc.view(-1, 1, d)[:n] = k, v
+    out = torch.empty_like(q)
+    lse = torch.empty(1, 1, device=DEV)
+    ops.attention_paged(q, kc, vc, torch.arange(pages, dtype=torch.int32, device=DEV)[None], _i32([n]), _i32([0, 1]), out, lse=lse)
+    # p = 2^(6 - 17) here: normal in fp16, so each is rounded at 2^-12 at most, and `keys * 2^-25` is not called upon
+    o, a, want = exact_rows(q, k, v, True, d ** -0.5)
+    assert ((out.double() - o).abs() <= 2.0 ** -12 * (o.abs() + a) + 2.0 ** -13 * a).all()
+    assert (lse.double() - want).abs().max() < 1e-5
