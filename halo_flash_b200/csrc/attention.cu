@@ -121,8 +121,8 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // The same barrier in the CTA of rank 0 of the cluster. What it tells of lies in tensor memory, or came by TMA; cluster-scope
-// acquire and release on every wait and arrival cost about 300 cycles each (a tile of 128 keys took 4000 cycles instead of
-// 2500) and order nothing more than that needs. Where a thread's own stores are meant, fence.acq_rel.cluster stands before.
+// acquire and release on every wait and arrival cost about 300 cycles each (4096 tokens: 234 us instead of 209) and order
+// nothing more than that needs. Where a thread's own stores are meant, fence.acq_rel.cluster stands before.
 __device__ __forceinline__ void bar_arrive_leader(unsigned long long* b) {
   asm volatile(
       "{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, 0;\n"
@@ -1345,10 +1345,13 @@ cudaError_t Launch(const AttnArgs& a, cudaStream_t s) {
   return LaunchKernel(attention_join_kernel<T, D, CG>, dim3(x, 4 * CG * parts), kJoinWarps * 32, 0, s, c, static_cast<uint32_t>(units));
 }
 
-// A pair's tile has twice the rows: it pays where a sequence's rows (tokens x heads of a group) fill more than one CTA's.
+// A pair's tile has twice the rows, and half of it is idle where a sequence's rows (tokens x heads of a group) do not fill
+// it: pairs from three CTAs' rows a sequence on. Measured, single CTA against pair, 8 sequences behind 4096 keys, 16/2 heads
+// of 256: 64 rows 26 / 50 us, 128 rows 34 / 45, 192 rows 40 / 45, 384 rows 47 / 48 (heads of 128: 33.5 / 32); one prompt of 4096
+// tokens 146 / 116; 8 single tokens over 2 GB 312 / 372.
 template <typename T, int D>
 cudaError_t LaunchPair(const AttnArgs& a, cudaStream_t s) {
-  if (static_cast<uint64_t>(a.tokens) * (a.q_heads / a.kv_heads) > static_cast<uint64_t>(a.batch) * kRows) return Launch<T, D, 2>(a, s);
+  if (static_cast<uint64_t>(a.tokens) * (a.q_heads / a.kv_heads) >= static_cast<uint64_t>(a.batch) * (3 * kRows)) return Launch<T, D, 2>(a, s);
   return Launch<T, D, 1>(a, s);
 }
 

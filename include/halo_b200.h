@@ -26,8 +26,9 @@
  *     halo_b200_norm_rope_qk_noalloc (per GPU, shared by its calls); (2) a device counter
  *     of staging waits that ran out (halo_b200_stage_timeouts; zero in normal
  *     operation); (3) the process-wide tuning switches of halo_b200_tune (host atomics,
- *     for experiments; production code never needs to touch them). Everything else is
- *     stateless and re-entrant.
+ *     for experiments; production code never needs to touch them); (4) on the host, the address
+ *     of the driver's tensor-map encoder and that the attention kernels' register counts have been
+ *     checked. Everything else is stateless and re-entrant.
  *   - Ordering: kernels are launched with programmatic stream serialization. A kernel reads
  *     and writes memory only after the kernel ahead of it in the stream has completed; while
  *     it waits for that it may already ask L2 to prefetch the input rows it was given (a hint

@@ -232,6 +232,16 @@ def test_one_long_sequence_is_split(hq, hk, d):
     paged([9000, 3, 30], [2, 1, 1], hq, hk, d, 64, BF16, seed=15)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hk,d,page", [(32, 2, 256, 8), (16, 1, 128, 64), (30, 2, 200, 256)])
+def test_many_rows_a_sequence(dtype, hq, hk, d, page):
+    """Groups of 15 and 16 heads: the batches whose tiles two CTAs share, with the edges of the ones above."""
+    paged([0, 0, 0, 0], [3, 40, 0, 200], hq, hk, d, page, dtype, seed=21, lens=[0, 7, 50, 150])
+    paged([9000, 3, 30], [40, 30, 20], hq, hk, d, page, dtype, seed=22)
+    paged([70, 5], [40, 31], hq, hk, d, page, dtype, seed=23, layout="both", causal=False, rows_behind=3)
+    packed([33, 0, 150, 5], hq, hk, d, dtype, seed=24)
+
+
 def test_same_call_gives_the_same_bits_and_shares_no_state():
     g, d = _gen(16), 128
     q, k, v = (_randn(g, 900, h, d, dtype=BF16) for h in (8, 2, 2))
