@@ -219,6 +219,8 @@ int RunAttention(AttnArgs a, uint64_t workspace_bytes, const char* what, halo_b2
   REQUIRE(a.workspace && Aligned(a.workspace, 16), "%s: the workspace is null or not 16-byte aligned", what);
   REQUIRE(workspace_bytes >= AttentionWorkspaceBytes(a.dim), "%s: the workspace has %llu bytes, %llu are needed", what,
           static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(AttentionWorkspaceBytes(a.dim)));
+  REQUIRE((a.tokens <= 1 || a.out_row >= a.dim) && (a.q_heads <= 1 || a.out_head >= a.dim), "%s: rows of out overlap", what);
+  REQUIRE(a.out != a.k && a.out != a.v, "%s: out must not be the memory of k or v", what);
   return Done(LaunchAttention(a, S(stream)), what, err, errlen);
 }
 
@@ -1655,6 +1657,7 @@ int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row
   a.dim = dim;
   a.page_shift = Log2(page_size);
   a.pages = pages;
+  REQUIRE(row_stride >= dim && (pages <= 1 || page_stride >= dim) && (heads <= 1 || head_stride >= dim), "%s: cache rows overlap", what);
   // strides of axes with one entry are never used
   const uint64_t odd = (tokens > 1 ? k_row_stride | v_row_stride : 0) | (heads > 1 ? k_head_stride | v_head_stride | head_stride : 0) |
                        (pages > 1 ? page_stride : 0) | row_stride | dim;

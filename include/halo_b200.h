@@ -525,6 +525,7 @@ int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table
  * [tokens][heads][dim] of `dtype` to the cache rows that slot names. Element (page, row, head, i) of either cache is
  * at page * page_stride + row * row_stride + head * head_stride + i. A slot that is negative or not below
  * pages * page_size is skipped. The slots of a call must differ: of two rows with the same slot either may remain.
+ * Cache rows must not overlap.
  * (dtype, cache_dtype) in (f32, f32|f16|bf16), (f16, f16|bf16), (bf16, bf16|f16). All strides are in elements. */
 int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row_stride, uint64_t k_head_stride,
                           const void* v, uint64_t v_row_stride, uint64_t v_head_stride, int dtype, void* k_cache,
@@ -543,7 +544,8 @@ uint64_t halo_b200_attention_workspace(uint32_t dim);
  *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * <q, k_j>),
  * over the sequence's rows j, up to the query's own when causal is 1. lse (optional, [tokens][q_heads]) =
  * log sum_j p_j. A query that sees no key gets zeros and -inf. Rows behind cu[batch] are neither read nor written.
- * cu rises from 0 and stays within tokens (what lies beyond is cut).
+ * cu rises from 0 and stays within tokens (what lies beyond is cut). Strides of 0 repeat a row or head of q, k or v;
+ * rows of out must not overlap. out may be q itself (same strides), and overlaps neither k nor v.
  * dtype f16 or bf16 for q, k, v and out; dim a multiple of 8 up to 256; q_heads / kv_heads a whole number up to 128;
  * scale > 0. Strides in elements, multiples of 8; pointers 16-byte aligned. Products are exact in fp32 sums; p is
  * rounded to dtype for the second product, out once from fp32. Values behind a mask never reach the result as long as

@@ -39,6 +39,18 @@ def test_attention_refuses(name, make, change, word):
     assert word in _fails(name, *make(**change))
 
 
+@pytest.mark.parametrize("name,make", [("attention_packed", _packed), ("attention_paged", _paged)])
+@pytest.mark.parametrize("change,word", [({"orow": 0}, "overlap"), ({"oh": 0}, "overlap"), ({"oh": 120}, "overlap"), ({"out": A}, "memory of"),
+                                         ({"out": 2 * A, "v": 2 * A}, "memory of")])
+def test_attention_refuses_outputs_that_overlap(name, make, change, word):
+    assert word in _fails(name, *make(**{"out": 3 * A, **change}))
+
+
+@pytest.mark.parametrize("ps,rs,hs", [(0, 128, 64), (8192, 0, 64), (8192, 128, 0), (8192, 56, 64)])
+def test_store_refuses_cache_rows_that_overlap(ps, rs, hs):
+    assert "overlap" in _fails("paged_store", A, 128, 64, A, 128, 64, 2, A, A, 2, ps, rs, hs, 3, 64, A, 2, 64, 5)
+
+
 def test_paged_attention_refuses():
     for change, word in (({"size": 48}, "page size"), ({"size": 4}, "page size"), ({"size": 512}, "page size"), ({"table": None}, "null"),
                          ({"kv": None}, "null"), ({"pages": 0}, "no pages"), ({"row": 260}, "strides"), ({"pages": 1 << 31}, "2^31")):

@@ -242,6 +242,22 @@ def test_many_rows_a_sequence(dtype, hq, hk, d, page):
     packed([33, 0, 150, 5], hq, hk, d, dtype, seed=24)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_broadcast_inputs_and_out_in_place_of_q(d):
+    """Strides of 0 repeat a row or head; out may be q. Both give the bits of the plain call."""
+    g, n = _gen(25), 700
+    q, k, v = (_randn(g, n, h, d, dtype=BF16) for h in (16, 1, 1))
+    cu = _i32([0, 100, n])
+    heads = [x.expand(n, 2, d) for x in (k, v)]
+    want = ops.attention_packed(q, *(x.contiguous() for x in heads), cu, torch.empty_like(q))
+    assert torch.equal(ops.attention_packed(q, *heads, cu, torch.empty_like(q)), want)
+    own = q.clone()
+    assert torch.equal(ops.attention_packed(own, *heads, cu, own), want)
+    rows = q[:1].expand(n, 16, d), k[:1].expand(n, 1, d)
+    want = ops.attention_packed(*(x.contiguous() for x in rows), v, cu, torch.empty_like(q))
+    assert torch.equal(ops.attention_packed(*rows, v, cu, torch.empty_like(q)), want)
+
+
 def test_same_call_gives_the_same_bits_and_shares_no_state():
     g, d = _gen(16), 128
     q, k, v = (_randn(g, 900, h, d, dtype=BF16) for h in (8, 2, 2))
