@@ -951,10 +951,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         float total = 0.0f;
         if (any) {
           wait(sh, l_full, l_phase);
-          // over the reference of the tile before the last one
-          const float other = *sl, others = before == ref ? other
-                                            : before == -INFINITY ? 0.0f
-                                                                  : __fmul_rn(other, ex2_approx(__fmul_rn(before - ref, c.scale_log2)));
+          // over the reference of the tile before the last one; without one it is 0, or NaN from scores that are NaN
+          const float other = *sl, others = before == ref || before == -INFINITY
+                                                ? other
+                                                : __fmul_rn(other, ex2_approx(__fmul_rn(before - ref, c.scale_log2)));
           pair_sync();
           if (half == 1) *sl = l;
           pair_sync();
@@ -1122,9 +1122,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
       c.lse[token * (c.kv_heads * c.group) + head] =
           total == 0.0f ? -INFINITY : __fmul_rn(__fmaf_rn(top, c.scale_log2, __log2f(total) - kLift<T>), 0.69314718055994531f);
   };
-  // a piece that saw nothing (weight 0) says nothing, whatever its sums are
+  // A piece without a maximum has no weight (-1): its sums say nothing. Its denominator does: 0, or NaN where its scores were
+  // NaN, which has no part in a maximum. A NaN denominator, behind a weight of 0 too, makes the joined one and so all outputs NaN.
   auto add = [](float4& sum, float w, float4 v) {
-    if (w != 0.0f) {
+    if (!(w < 0.0f)) {
       sum.x = __fmaf_rn(w, v.x, sum.x);
       sum.y = __fmaf_rn(w, v.y, sum.y);
       sum.z = __fmaf_rn(w, v.z, sum.z);
@@ -1132,7 +1133,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
     }
   };
   auto quad = [&](uint32_t p, uint32_t q) { return *reinterpret_cast<const float4*>(piece(p) + (q * kRows + row) * 4); };
-  auto weight = [&](float r, float top) { return r == -INFINITY ? 0.0f : ex2_approx(__fmul_rn(r - top, c.scale_log2)); };
+  auto weight = [&](float r, float top) { return r == -INFINITY ? -1.0f : ex2_approx(__fmul_rn(r - top, c.scale_log2)); };
 
   if (pieces <= kFew) {
     float r[kFew], l[kFew], top = -INFINITY, total = 0.0f;
@@ -1155,7 +1156,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
 #pragma unroll
         for (uint32_t p = 0; p < kFew; ++p) {
           r[p] = weight(r[p], top);
-          if (r[p] != 0.0f) total = __fmaf_rn(r[p], l[p], total);
+          total = __fmaf_rn(fabsf(r[p]), l[p], total);
         }
       }
       const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
@@ -1188,8 +1189,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, kJoinResident) attention_join
   __syncthreads();
 #pragma unroll 4
   for (uint32_t p = warp; p < pieces; p += kJoinWarps) {
-    const float w = weight(ref(p), top);
-    if (w != 0.0f) total = __fmaf_rn(w, piece(p)[(D + 1) * kRows + row], total);
+    const float l = mine ? piece(p)[(D + 1) * kRows + row] : 0.0f;
+    total = __fmaf_rn(fabsf(weight(ref(p), top)), l, total);
   }
   meet[warp][lane] = total;
   __syncthreads();

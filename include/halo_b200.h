@@ -549,8 +549,8 @@ uint64_t halo_b200_attention_workspace(uint32_t dim);
  * dtype f16 or bf16 for q, k, v and out; dim a multiple of 8 up to 256; q_heads / kv_heads a whole number up to 128;
  * scale > 0. Strides in elements, multiples of 8; pointers 16-byte aligned. Products are exact in fp32 sums; p is
  * rounded to dtype for the second product, out once from fp32. Values behind a mask never reach the result as long as
- * they are finite; a V row that is not finite reaches the queries of a tile in which some query sees it. The same call
- * gives the same bits. */
+ * they are finite; a V row that is not finite reaches the queries of a tile in which some query sees it. A query that sees a
+ * score of NaN gets NaN, in out and in lse. The same call gives the same bits. */
 int halo_b200_attention_packed(halo_b200_stream stream, const void* q, uint64_t q_row_stride, uint64_t q_head_stride,
                                const void* k, uint64_t k_row_stride, uint64_t k_head_stride, const void* v,
                                uint64_t v_row_stride, uint64_t v_head_stride, void* out, uint64_t out_row_stride,
