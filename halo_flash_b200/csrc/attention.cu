@@ -31,6 +31,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "softmax_pair.cuh"
 #include "stage.cuh"
 
 namespace halo_b200 {
@@ -75,7 +76,6 @@ struct Shape {
   static constexpr uint32_t kQBufs = D <= 128 ? 2 : 1;
   static constexpr bool kDrain = kQBufs == 1;
   static constexpr uint32_t kSlots = kDrain ? 2 : 4;     // references and denominators in flight between the two pairs
-  static constexpr uint32_t kMaxSlots = kDrain ? 1 : 2;  // maxima in flight between the groups of a pair
 };
 
 struct alignas(16) Basics {
@@ -89,8 +89,8 @@ struct alignas(16) Shared : Basics {
   unsigned long long s_full[Sh::kBufs], p_full[Sh::kBufs][2], pv_done[Sh::kBufs], o_empty, v_dirty, v_clean;
   unsigned long long m_full[Sh::kSlots][4], l_full[Sh::kSlots][4];
   float l[Sh::kSlots][kRows];
-  float m[Sh::kSlots][kRows];            // references
-  float mx[2][Sh::kMaxSlots][2][kRows];  // maxima of a pair's two groups
+  float m[Sh::kSlots][kRows];  // references
+  PairTrade<kRows> trade[2][kPairTrades];  // what a pair's two groups tell each other
 };
 template <int D, int CG>
 constexpr uint32_t kSmemBytes =
@@ -839,11 +839,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (uint32_t x = 0; x < HK / 32; ++x) tc_ld32(tmem + lane_base + buf * KT + half * HK + x * 32u, s[x]);
           float ref = -INFINITY;  // the other pair's, of the tile before
-          if (t > pc.t0) {
+          if (half == 0 && t > pc.t0) {
             wait(sh, &sh.m_full[(g - 1) % NS][quad], ((g - 1) / NS) & 1u);
             ref = sh.m[(g - 1) % NS][row];
           }
-          before = ref;
           tc_wait_ld(s);
           const uint32_t key0 = t * KT + half * HK;
           if (key0 + HK > min(all_see, pc.keys)) {
@@ -861,12 +860,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (uint32_t x = 0; x < HK; x += 2) part[x / 2 % 4] = max3f(part[x / 2 % 4], s[x / 32][x % 32], s[x / 32][x % 32 + 1]);
           float mx = fmaxf(max3f(part[0], part[1], part[2]), part[3]);
           if (row >= rows) mx = -INFINITY;  // no query row: what stands there has no say
-          float* trade = sh.mx[pair][(g >> 1) % Sh::kMaxSlots][0];
-          trade[half * kRows + row] = mx;
-          tc_before();  // behind this P of either group may replace S
-          pair_sync();
-          tc_after();
-          mx = fmaxf(trade[row], trade[kRows + row]);
+          trade_maxima(sh.trade[pair][trade_of(g)], half, row, mx, ref, [&] {
+            tc_before();  // behind this P of either group may replace S
+            pair_sync();
+            tc_after();
+          });
+          before = ref;
           // the reference follows where it has fallen too far behind
           const float grown = __fmul_rn(mx - ref, c.scale_log2);
           const bool follow = grown > kLazy;  // also from -inf; false for -inf against -inf (NaN)
