@@ -26,6 +26,9 @@
 //
 // Waits are bounded as in stage.cuh: one that runs out sets a flag that makes the other waits return at once, the CTA
 // finishes its control flow without storing, and the count is reported by halo_b200_stage_timeouts.
+// Barriers without a bound are those that every thread passes equally often whatever the waits said: the one of a pair of
+// softmax groups (softmax_pair.cuh) and the CTA's or cluster's at the start and the end. The last one comes after all copies
+// and products have landed: also those that were issued behind a wait that had run out.
 #include "attention.cuh"
 
 #include <atomic>
@@ -80,6 +83,7 @@ struct Shape {
 
 struct alignas(16) Basics {
   uint32_t tmem, abort;
+  unsigned long long drained;  // after a wait has run out: the products issued until then are done
   uint32_t start[4], end[4];  // (sequence, K/V head, row tile, key tile) of the piece's borders
 };
 template <int D, int CG>
@@ -529,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (uint32_t i = 0; i < NS; ++i)
       for (int w = 0; w < 4; ++w) bar_init(&sh.m_full[i][w], 1), bar_init(&sh.l_full[i][w], 1);
+    bar_init(&sh.drained, 1);
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1036,9 +1041,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   __syncwarp();
+  if constexpr (CG == 2) {  // a pair's CTAs end alike: the products use the operands and barriers of both
+    if (lane == 0 && aborted(sh))
+      asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nst.shared::cluster.u32 [r], %2;\n}" ::"r"(smem_addr(&sh.abort)),
+                   "r"(rank ^ 1u), "r"(1u)
+                   : "memory");
+    __syncwarp();
+  }
   tc_before();
   sync_all<CG>();
   tc_after();
+  if (aborted(sh)) {  // nobody waits any more, so all threads of both CTAs see the same
+    if (warp == kSoftmaxWarps + 1 && rank == 0 && elect()) tc_commit<CG>(&sh.drained);
+    if (threadIdx.x == 0) stage_wait(smem_addr(&sh.drained), 0);
+    __syncwarp();
+    sync_all<CG>();
+  }
   if (warp == kSoftmaxWarps + 1) {
     if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
