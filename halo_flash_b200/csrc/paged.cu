@@ -180,7 +180,8 @@ cudaError_t LaunchStore(const StoreArgs& a, cudaStream_t s) {
 cudaError_t LaunchPagedPlan(const PlanArgs& a, cudaStream_t s) {
   const unsigned smem = 8u * (a.batch + 1);
   if (smem > 48u * 1024u) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // for the largest batch, always: calls from several threads set the same limit, none one that is too low for another's launch
+    const cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(8u * (kMaxPlanBatch + 1)));
     if (e != cudaSuccess) return e;
   }
   // new pages <= tokens + batch, but `tokens` may be shorter than the lengths say; the loops stride, so any grid is right
