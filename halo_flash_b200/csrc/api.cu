@@ -9,6 +9,7 @@
 
 #include "../../include/halo_b200.h"
 #include "kernels.h"
+#include "overlap.h"
 
 using namespace halo_b200;
 
@@ -219,8 +220,16 @@ int RunAttention(AttnArgs a, uint64_t workspace_bytes, const char* what, halo_b2
   REQUIRE(a.workspace && Aligned(a.workspace, 16), "%s: the workspace is null or not 16-byte aligned", what);
   REQUIRE(workspace_bytes >= AttentionWorkspaceBytes(a.dim), "%s: the workspace has %llu bytes, %llu are needed", what,
           static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(AttentionWorkspaceBytes(a.dim)));
-  REQUIRE((a.tokens <= 1 || a.out_row >= a.dim) && (a.q_heads <= 1 || a.out_head >= a.dim), "%s: rows of out overlap", what);
-  REQUIRE(a.out != a.k && a.out != a.v, "%s: out must not be the memory of k or v", what);
+  // CTAs write their rows in no order, while others read
+  const uint64_t run = a.dim * 2ull, key_rows = a.table ? uint64_t{1} << a.page_shift : a.tokens, key_pages = a.table ? a.pages : 1;
+  const View out = View(a.out, run).Along(a.tokens, a.out_row, 2).Along(a.q_heads, a.out_head, 2);
+  REQUIRE(!OverlapsItself(out), "%s: rows of out overlap", what);
+  REQUIRE(!Overlap(out, View(a.k, run).Along(key_rows, a.k_row, 2).Along(a.kv_heads, a.k_head, 2).Along(key_pages, a.k_page, 2)) &&
+              !Overlap(out, View(a.v, run).Along(key_rows, a.v_row, 2).Along(a.kv_heads, a.v_head, 2).Along(key_pages, a.v_page, 2)),
+          "%s: out must not be in the memory of k or v", what);
+  const bool in_place = a.out == a.q && (a.tokens <= 1 || a.out_row == a.q_row) && (a.q_heads <= 1 || a.out_head == a.q_head);
+  REQUIRE(in_place || !Overlap(out, View(a.q, run).Along(a.tokens, a.q_row, 2).Along(a.q_heads, a.q_head, 2)),
+          "%s: out is in the memory of q, but is not q", what);
   return Done(LaunchAttention(a, S(stream)), what, err, errlen);
 }
 
@@ -1597,13 +1606,18 @@ int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table
   REQUIRE(n_free == 0 || free_pages, "%s: the free list is null", what);
   REQUIRE(n_free < (1u << 31) && tokens < (1u << 31), "%s: more than 2^31 pages or tokens", what);
   REQUIRE(table_stride >= table_cols || batch <= 1, "%s: table rows overlap", what);
-  // every CTA reads the lengths while one writes kv_len and cu
-  REQUIRE(batch == 0 || ((kv_len == nullptr || (kv_len != past && kv_len != fresh)) && (cu == nullptr || (cu != past && cu != fresh))),
-          "%s: an output must not be the memory of past or fresh", what);
   REQUIRE(Aligned(table, 4) && Aligned(past, 4) && Aligned(fresh, 4) && Aligned(free_pages, 4) && Aligned(slot, 8) &&
               Aligned(pos, 4) && Aligned(cu, 4) && Aligned(kv_len, 4) && Aligned(status, 4),
           "%s: pointer not aligned to its element type", what);
   if (batch == 0 && tokens == 0 && !cu && !status) return Done(cudaSuccess, what, err, errlen);
+  // every CTA reads the lengths and the free list while others write
+  const View in[] = {View(past, batch * 4ull), View(fresh, batch * 4ull), View(free_pages, n_free * 4ull)};
+  const View to[] = {View(table, table_cols * 4ull).Along(batch, table_stride, 4), View(slot, tokens * 8ull), View(pos, pos ? tokens * 4ull : 0),
+                     View(cu, cu ? (batch + 1) * 4ull : 0), View(kv_len, kv_len ? batch * 4ull : 0), View(status, status ? 12 : 0)};
+  for (const View& o : to)
+    for (const View& i : in) REQUIRE(!Overlap(o, i), "%s: an output must not be in the memory of past, fresh or free_pages", what);
+  for (const View& o : to)
+    for (const View* i = &o + 1; i != to + 6; ++i) REQUIRE(!Overlap(o, *i), "%s: two outputs share memory", what);
   PlanArgs a{};
   a.table = table;
   a.table_stride = table_stride;
@@ -1657,14 +1671,17 @@ int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row
   a.dim = dim;
   a.page_shift = Log2(page_size);
   a.pages = pages;
-  REQUIRE(row_stride >= dim && (pages <= 1 || page_stride >= dim) && (heads <= 1 || head_stride >= dim), "%s: cache rows overlap", what);
+  REQUIRE(dtype == kF32 || cache_dtype != kF32, "%s: unsupported (rows, cache) dtype combination", what);
+  const auto cache = [&](const void* p) {
+    return View(p, dim * ds).Along(page_size, row_stride, ds).Along(heads, head_stride, ds).Along(pages, page_stride, ds);
+  };
+  REQUIRE(!OverlapsItself(cache(k_cache)), "%s: cache rows overlap", what);
+  REQUIRE(!Overlap(cache(k_cache), cache(v_cache)), "%s: k_cache and v_cache overlap", what);
   // strides of axes with one entry are never used
   const uint64_t odd = (tokens > 1 ? k_row_stride | v_row_stride : 0) | (heads > 1 ? k_head_stride | v_head_stride | head_stride : 0) |
                        (pages > 1 ? page_stride : 0) | row_stride | dim;
   a.vec = odd % 8 == 0 && Aligned(k, 16) && Aligned(v, 16) && Aligned(k_cache, 16) && Aligned(v_cache, 16);
-  const cudaError_t e = LaunchPagedStore(a, S(stream));
-  if (e == cudaErrorInvalidValue) return Fail(err, errlen, "%s: unsupported (rows, cache) dtype combination", what);
-  return Done(e, what, err, errlen);
+  return Done(LaunchPagedStore(a, S(stream)), what, err, errlen);
 }
 
 uint64_t halo_b200_attention_workspace(uint32_t dim) { return AttentionWorkspaceBytes(dim); }

@@ -514,8 +514,8 @@ int halo_b200_scale_silu(halo_b200_stream stream, const float* x, void* y, int y
  * A request that needs more than table_cols pages, or whose pages would pass the end of the free list, is refused: it
  * takes no page, its slots are -1 and its kv_len stays past[r]. Requests are served in order: once the list cannot
  * serve one, it serves none behind it that needs a page. slot and pos have `tokens` entries: those behind the last
- * new token get -1 and 0, new tokens beyond them get none. batch <= 16384, n_free < 2^31, lengths < 2^31. No output may
- * lie in the memory of past, fresh or free_pages (a step's kv_len goes to a second buffer). */
+ * new token get -1 and 0, new tokens beyond them get none. batch <= 16384, n_free < 2^31, lengths < 2^31. Outputs
+ * that lie in the memory of past, fresh or free_pages (a step's kv_len goes to a second buffer) or of each other are refused. */
 int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table_stride, uint32_t table_cols,
                          const uint32_t* past, const uint32_t* fresh, const int32_t* free_pages, uint32_t n_free,
                          uint32_t page_size, int64_t* slot, uint32_t* pos, uint32_t* cu, uint32_t* kv_len,
@@ -525,7 +525,7 @@ int halo_b200_paged_plan(halo_b200_stream stream, int32_t* table, uint64_t table
  * [tokens][heads][dim] of `dtype` to the cache rows that slot names. Element (page, row, head, i) of either cache is
  * at page * page_stride + row * row_stride + head * head_stride + i. A slot that is negative or not below
  * pages * page_size is skipped. The slots of a call must differ: of two rows with the same slot either may remain.
- * Cache rows must not overlap.
+ * Cache rows that overlap, of one cache or of both, are refused. k and v may lie in a cache as long as no slot names a row of them.
  * (dtype, cache_dtype) in (f32, f32|f16|bf16), (f16, f16|bf16), (bf16, bf16|f16). All strides are in elements. */
 int halo_b200_paged_store(halo_b200_stream stream, const void* k, uint64_t k_row_stride, uint64_t k_head_stride,
                           const void* v, uint64_t v_row_stride, uint64_t v_head_stride, int dtype, void* k_cache,
@@ -544,8 +544,8 @@ uint64_t halo_b200_attention_workspace(uint32_t dim);
  *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * <q, k_j>),
  * over the sequence's rows j, up to the query's own when causal is 1. lse (optional, [tokens][q_heads]) =
  * log sum_j p_j. A query that sees no key gets zeros and -inf. Rows behind cu[batch] are neither read nor written.
- * cu rises from 0 and stays within tokens (what lies beyond is cut). Strides of 0 repeat a row or head of q, k or v;
- * rows of out must not overlap. out may be q itself (same strides), and overlaps neither k nor v.
+ * cu rises from 0 and stays within tokens (what lies beyond is cut). Strides of 0 repeat a row or head of q, k or v.
+ * out may be q itself (same strides); an out that overlaps q in another way, k, v, or itself is refused.
  * dtype f16 or bf16 for q, k, v and out; dim a multiple of 8 up to 256; q_heads / kv_heads a whole number up to 128;
  * scale > 0. Strides in elements, multiples of 8; pointers 16-byte aligned. Products are exact in fp32 sums; p is
  * rounded to dtype for the second product, out once from fp32. Values behind a mask never reach the result as long as
