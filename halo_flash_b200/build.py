@@ -51,18 +51,28 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 
 
 def _build_bind(nvcc: str, force: bool) -> None:
-    src = CSRC / "bind.cpp"
-    if not force and not _stale(BIND, [src, INCLUDE / "halo_b200.h", Path(__file__)]):
+    """The extension module, where Python's and torch's headers are; a C or C++ program needs neither."""
+    spec = find_spec("torch")
+    headers = Path(sysconfig.get_paths()["include"])
+    if spec is None or not (headers / "Python.h").exists():
+        print(f"[build] no {'torch' if spec is None else headers / 'Python.h'}: {BIND.name}, through which ops.py makes its attention calls, is not built",
+              file=sys.stderr)
         return
-    torch = Path(find_spec("torch").submodule_search_locations[0])
+    src = CSRC / "bind.cpp"
+    torch = Path(spec.submodule_search_locations[0])
     cuda = Path(nvcc).resolve().parents[1]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(INCLUDE), "-I", sysconfig.get_paths()["include"],
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(INCLUDE), "-I", str(headers),
            "-isystem", str(torch / "include"), "-isystem", str(torch / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
            str(src), "-o", str(BIND), "-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
            "-L", str(PKG), "-lhalo_b200", "-Wl,-rpath,$ORIGIN"]
+    # a module built against another torch or Python does not load
+    made_with, stamp = "\n".join([*cmd, sys.version, (torch / "version.py").read_text()]), OBJ / "bind.stamp"
+    if not force and not _stale(BIND, [src, INCLUDE / "halo_b200.h", Path(__file__)]) and stamp.exists() and stamp.read_text() == made_with:
+        return
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"g++ failed on bind.cpp:\n{p.stdout}\n{p.stderr}")
+    stamp.write_text(made_with)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

@@ -336,7 +336,7 @@ def _bind():
         try:
             from . import _bind as module
         except ImportError as e:
-            raise FileNotFoundError("halo_flash_b200/_bind is missing or does not load: build it with "
+            raise FileNotFoundError(f"halo_flash_b200/_bind is missing or does not load ({e}): build it with "
                                     "`python -m halo_flash_b200.build`") from e
         _bound = module
     return _bound
