@@ -161,7 +161,13 @@ class Library:
         self.cdll.halo_b200_launch.restype = C.c_int
         self.cdll.halo_b200_launch.argtypes = [_p, C.c_char_p, C.POINTER(HaloArg), _sz, C.POINTER(C.c_uint32 * 3),
                                                C.POINTER(C.c_uint32 * 3), C.c_char_p, _sz]
-        self.calls = 0  # kernel-launching calls made through this binding (for launch accounting)
+        self._calls = 0
+        self.counters = []  # of the calls that another module makes of the same entry points
+
+    @property
+    def calls(self) -> int:
+        """Kernel-launching calls made of the library's entry points (for launch accounting)."""
+        return self._calls + sum(count() for count in self.counters)
 
     def version(self) -> str:
         return self.cdll.halo_b200_version().decode()
@@ -180,7 +186,7 @@ class Library:
         except AttributeError:
             err = self._local.err = C.create_string_buffer(512)
         rc = self._fn[name](stream, *args, err, 512)
-        self.calls += 1
+        self._calls += 1
         if rc != 0:
             raise HaloError(err.value.decode(errors="replace"))
 
@@ -190,7 +196,7 @@ class Library:
         b = (C.c_uint32 * 3)(*block)
         err = C.create_string_buffer(512)
         rc = self.cdll.halo_b200_launch(stream, name.encode(), arr, len(args), C.byref(g), C.byref(b), err, len(err))
-        self.calls += 1
+        self._calls += 1
         if rc != 0:
             raise HaloError(err.value.decode(errors="replace"))
 

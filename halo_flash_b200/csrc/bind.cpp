@@ -149,7 +149,10 @@ Table GetTable(PyObject* o) {
   return r;
 }
 
+unsigned long long g_calls = 0;  // of the C ABI's entry points, under the interpreter's lock
+
 void Done(int rc, const char* err) {
+  ++g_calls;
   if (rc != 0) Refuse(nullptr, "%s", err);
 }
 
@@ -302,9 +305,11 @@ PyObject* AttentionPaged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+PyObject* Calls(PyObject*, PyObject*) { return PyLong_FromUnsignedLongLong(g_calls); }
+
 #define HALO_METHOD(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {HALO_METHOD("paged_plan", PagedPlan), HALO_METHOD("paged_store", PagedStore), HALO_METHOD("attention_packed", AttentionPacked),
-                          HALO_METHOD("attention_paged", AttentionPaged), {nullptr, nullptr, 0, nullptr}};
+                          HALO_METHOD("attention_paged", AttentionPaged), {"calls", Calls, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", "The paged-cache and attention calls on torch tensors; see ops.py.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
 

@@ -338,6 +338,7 @@ def _bind():
         except ImportError as e:
             raise FileNotFoundError(f"halo_flash_b200/_bind is missing or does not load ({e}): build it with "
                                     "`python -m halo_flash_b200.build`") from e
+        lib().counters.append(module.calls)
         _bound = module
     return _bound
 
