@@ -206,7 +206,8 @@ int RunAttention(AttnArgs a, uint64_t workspace_bytes, const char* what, halo_b2
   REQUIRE(a.kv_heads > 0 && a.q_heads > 0 && a.q_heads % a.kv_heads == 0, "%s: q_heads %u is no multiple of kv_heads %u", what,
           a.q_heads, a.kv_heads);
   REQUIRE(a.q_heads / a.kv_heads <= 128, "%s: more than 128 query heads for each K/V head", what);
-  REQUIRE(std::isfinite(a.scale) && a.scale > 0.0f, "%s: scale must be positive and finite", what);
+  // the kernels multiply by scale log2(e)
+  REQUIRE(a.scale > 0.0f && std::isfinite(static_cast<float>(a.scale * 1.4426950408889634)), "%s: scale must be positive and finite (times log2 e)", what);
   REQUIRE(a.causal == 0 || a.causal == 1, "%s: causal must be 0 or 1", what);
   REQUIRE(a.tokens < (1u << 31) && a.batch < (1u << 31), "%s: more than 2^31 tokens or sequences", what);
   REQUIRE(Aligned(a.q, 16) && Aligned(a.k, 16) && Aligned(a.v, 16) && Aligned(a.out, 16), "%s: pointer not 16-byte aligned", what);

@@ -547,7 +547,7 @@ uint64_t halo_b200_attention_workspace(uint32_t dim);
  * cu rises from 0 and stays within tokens (what lies beyond is cut). Strides of 0 repeat a row or head of q, k or v.
  * out may be q itself (same strides); an out that overlaps q in another way, k, v, or itself is refused.
  * dtype f16 or bf16 for q, k, v and out; dim a multiple of 8 up to 256; q_heads / kv_heads a whole number up to 128;
- * scale > 0. Strides in elements, multiples of 8; pointers 16-byte aligned. Products are exact in fp32 sums; p is
+ * scale > 0, below 2.3e38. Strides in elements, multiples of 8; pointers 16-byte aligned. Products are exact in fp32 sums; p is
  * rounded to dtype for the second product, out once from fp32. Values behind a mask never reach the result as long as
  * they are finite; a V row that is not finite reaches the queries of a tile in which some query sees it. A query that sees a
  * score of NaN gets NaN, in out and in lse. The same call gives the same bits. */
