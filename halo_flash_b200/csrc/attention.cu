@@ -4,8 +4,8 @@
 // Mathematics. A tile is 128 query rows against KT keys. S = Q K^T goes to TMEM in fp32; each row keeps a
 // reference r (near its running maximum) and l = sum of p, p = 2^(c s - c r), c = scale log2 e; O += P V stays in
 // TMEM in fp32, and at the end O / l is rounded once. Any reference gives the same result, so r follows the maximum
-// only when that has grown by more than 2^8: until then p stays below 2^8, which neither bf16 nor fp16 nor the fp32
-// sums mind, and O need not be rescaled. P is rounded to the inputs' 16-bit type for the tensor cores (as every
+// only when that has grown by more than 2^8: until then p stays below 2^8 (2^14 in fp16, where all p carry a factor 2^6:
+// kLift), which neither type nor the fp32 sums mind, and O need not be rescaled. P is rounded to the inputs' 16-bit type for the tensor cores (as every
 // output is), l is summed from the unrounded p.
 //
 // Rows. The group of query heads that share a K/V head is folded into the rows: row r of a tile is token r / G, head
@@ -49,10 +49,13 @@ constexpr uint32_t kThreads = 640, kSoftmaxWarps = 16;
 // which hold half a row of S: 4 x 128 x 104 + 128 x 64 = 640 x 96.
 constexpr uint32_t kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
 static_assert(512 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "a share above the launch's total would wait for good");
-// What a job costs beside its key tiles, in key tiles (4096 tokens, 16/2 heads of 256: 121 us with 1, 115 with 2, 116 with 3, 117 with 4).
+// What a job costs beside its key tiles, in key tiles. Measured with 1, 2, 3 and 4: 4096 tokens, 16/2 heads of 256: 123, 116, 119,
+// 118 us; 8192 tokens, 16/4 heads of 128: 247, 231, 227, 228; of 64: 237, 213, 214, 217; 9 prompts of 5003 tokens: 47.6, 45.4, 44.9,
+// 45.2; 24 sessions with 700 new tokens: 84.9, 85.6, 86.5, 87.0.
 constexpr uint32_t kJobCost = 2;
 constexpr uint32_t kSnap = 1;      // a border within so many tiles of a job's end moves to that end
-// Least share of a unit, job costs counted (one token over 1501 keys: 15.2 us with 1, 14.9 with 2, 14.2 with 3, 14.9 with 4).
+// Least share of a unit, job costs counted. Measured with 1, 2, 3 and 4: one token over 1501 keys 14.7, 14.2, 14.0, 14.6 us; 4 over
+// 513 keys 15.3, 15.2, 15.7, 16.1; 8 over 2049 21.1, 21.0, 21.2, 20.8; 2 over 4097, 32/8 heads of 128: 20.5, 20.6, 20.6, 20.4.
 constexpr uint32_t kMinShare = 3;
 constexpr uint32_t kMaxCtas = 148;
 constexpr float kLazy = 8.0f;      // log2 of the growth that a reference may lag behind
@@ -300,7 +303,8 @@ __device__ __forceinline__ uint32_t key_end(const AttnCall& c, const Seq& s, uin
   const int e = s.off + static_cast<int>(min(s.rows, (i + 1) * tq));
   return e > 0 ? static_cast<uint32_t>(e) : 0u;
 }
-// sum over i < n of floor((a i + b) / M) for a power of two M, by Euclid's algorithm on (a, M). a n + b < 2^32.
+// sum over i < n of floor((a i + b) / M) for a power of two M. a n + b < 2^32. The well-known count of the lattice points
+// under a line: the parts that divide are taken out, the axes trade places, as in Euclid's algorithm on (a, M).
 template <uint32_t M>
 __device__ __forceinline__ unsigned long long floor_sum(uint32_t n, uint32_t a, uint32_t b) {
   auto pairs = [](uint32_t k) { return static_cast<unsigned long long>(k) * (k - 1) / 2; };
@@ -1376,6 +1380,7 @@ cudaError_t LaunchPair(const AttnArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t LaunchDim(const AttnArgs& a, cudaStream_t s) {
   switch (PadDim(a.dim)) {
+    // no pair at 64: its second CTA would stage half of V's columns, and 64 of them are one 128-byte swizzled chunk
     case 64: return Launch<T, 64, 1>(a, s);
     case 128: return LaunchPair<T, 128>(a, s);
     default: return LaunchPair<T, 256>(a, s);

@@ -15,7 +15,7 @@ namespace {
 // launch, no atomics and no second pass: every CTA reads all lengths and builds the two prefix sums (tokens, new
 // pages) in its own shared memory, then takes its share of the tokens and of the new pages, each of which finds
 // its request by bisection. A token of a new page takes the page from the free list itself, not from the table that
-// some other CTA is writing.
+// some other CTA is writing. 8 requests 2.5 us, 1024 requests with 65536 tokens 4.4 us.
 constexpr unsigned kPlanThreads = 512;
 
 // The first index whose entry is greater than x, less one (a[0] == 0 <= x).
@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
 
 // ---- store ------------------------------------------------------------------------------------------------
 // HBM bound: each row is read once and written once. A thread moves one octet (8 values) of K and the same octet of
-// V, both loads in flight before either store; neighbouring threads take neighbouring octets of a row.
+// V, both loads in flight before either store; neighbouring threads take neighbouring octets of a row. 65536 rows of
+// 2 x 256: 42.9 us from 16-bit to 16-bit types (6.3 TB/s), 62.0 from fp32 to bf16 (6.5), 86.8 from fp32 to fp32 (6.2).
 template <typename IT, typename OT, bool VEC>
 __global__ void __launch_bounds__(kBlock) paged_store_kernel(const StoreArgs a) {
   pdl_begin();
